@@ -10,6 +10,18 @@
 
 #include "../../include/gq_hip.h"
 
+/* ---- context (gq_runtime.hip) ------------------------------------------ */
+struct GqCtxInfo {
+  int dev, n_cu;
+  hipStream_t stream;
+};
+GqCtxInfo gq_ctx_info(const gq_ctx *c);
+/* sets the context's error message and returns code */
+int gq_ctx_fail(gq_ctx *c, int code, const char *msg);
+/* the context's workspace of the paged entry points, at least so many bytes;
+ * it only grows, behind the work that still uses it.  NULL: no memory. */
+void *gq_ctx_paged_ws(gq_ctx *c, size_t bytes);
+
 /* ---- quantised matvec ----------------------------------------------------
  * One launch computes up to three row segments of the same dtype and shared
  * input x (e.g. the q and k projections), with optional fused prologue and

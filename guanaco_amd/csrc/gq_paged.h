@@ -1,0 +1,92 @@
+/*
+ * gq_paged.h — what the kernels over the paged K/V cache share
+ * (gq_paged.hip).
+ */
+#ifndef GQ_PAGED_H
+#define GQ_PAGED_H
+
+#include "gq_device.h"
+#include "gq_internal.h"
+
+typedef float gq_f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 gq_bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 gq_bf16x8 __attribute__((ext_vector_type(8)));
+
+/* gq_pages and gq_batch as the kernels take them */
+struct PgdPages {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int n_pages, lg, n_kv; /* 1 << lg positions a page */
+};
+struct PgdBatch {
+  const int32_t *table, *pos, *first;
+  int n_seqs, stride, n_tokens, max_len;
+};
+
+constexpr int pgd_bytes(int dtype) { return dtype == GQ_F32 ? 4 : dtype == GQ_BF16 ? 2 : 1; }
+
+/* The sequence of packed row t (uniform in the wave, all lanes active): the
+ * last s with first[s] <= t, so that the row lies before first[s + 1]; n_seqs
+ * where it belongs to none.  64 sequences a step. */
+__device__ __forceinline__ int pgd_seq_of(const PgdBatch &b, int t) {
+  if (!b.first) return t < b.n_seqs ? t : b.n_seqs;
+  const int lane = threadIdx.x & 63;
+  for (int s0 = 0; s0 < b.n_seqs; s0 += GQ_WAVE) {
+    const int s = s0 + lane;
+    const uint64_t after = __ballot(s < b.n_seqs && gld<int>(b.first + min(s, b.n_seqs - 1) + 1) > t);
+    if (after) return s0 + __builtin_ctzll(after);
+  }
+  return b.n_seqs;
+}
+
+/* (row of the first new token, their number); none where the rows are not in
+ * the packed arrays */
+__device__ __forceinline__ int2 pgd_rows(const PgdBatch &b, int s) {
+  if (!b.first) return make_int2(s, s < b.n_tokens ? 1 : 0);
+  const int r0 = gld<int>(b.first + s), r1 = gld<int>(b.first + s + 1);
+  return r0 < 0 || r1 > b.n_tokens || r1 <= r0 ? make_int2(0, 0) : make_int2(r0, r1 - r0);
+}
+
+/* Page of position p of sequence s; -1: it does not exist. */
+__device__ __forceinline__ int pgd_page(const PgdPages &c, const PgdBatch &b, int s, int p) {
+  const int i = p >> c.lg;
+  if (p < 0 || p >= b.max_len || i >= b.stride) return -1;
+  const int page = gld<int>(b.table + (size_t)s * b.stride + i);
+  return (unsigned)page < (unsigned)c.n_pages ? page : -1;
+}
+/* row of (page, head, slot) in a pool */
+__device__ __forceinline__ size_t pgd_row(const PgdPages &c, int page, int head, int slot) {
+  return (((size_t)page * c.n_kv + head) << c.lg) + slot;
+}
+
+/* two floats to bf16, nearest even */
+__device__ __forceinline__ uint32_t pgd_pack(float x, float y) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x, y}, gq_bf16x2));
+}
+__device__ __forceinline__ float pgd_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+__device__ __forceinline__ float pgd_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+
+/* eight consecutive values of GQ_F32 or GQ_BF16, and back */
+template <int T>
+__device__ __forceinline__ void pgd_load8(const void *base, size_t at, float (&x)[8]) {
+  if constexpr (T == GQ_F32) {
+    const float4 a = gld<float4>((const float *)base + at), b = gld<float4>((const float *)base + at + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const uint4 w = gld<uint4>((const uint16_t *)base + at);
+    x[0] = pgd_lo(w.x), x[1] = pgd_hi(w.x), x[2] = pgd_lo(w.y), x[3] = pgd_hi(w.y);
+    x[4] = pgd_lo(w.z), x[5] = pgd_hi(w.z), x[6] = pgd_lo(w.w), x[7] = pgd_hi(w.w);
+  }
+}
+template <int T>
+__device__ __forceinline__ void pgd_store8(void *base, size_t at, const float (&x)[8]) {
+  if constexpr (T == GQ_F32) {
+    gst<float4>((float *)base + at, make_float4(x[0], x[1], x[2], x[3]));
+    gst<float4>((float *)base + at + 4, make_float4(x[4], x[5], x[6], x[7]));
+  } else {
+    gst<uint4>((uint16_t *)base + at, make_uint4(pgd_pack(x[0], x[1]), pgd_pack(x[2], x[3]), pgd_pack(x[4], x[5]), pgd_pack(x[6], x[7])));
+  }
+}
+
+#endif

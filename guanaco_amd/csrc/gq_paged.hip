@@ -1,0 +1,631 @@
+/*
+ * gq_paged.hip — a K/V cache in pages that many sequences share: rows appended
+ * and read back, and attention over them (gfx950).
+ *
+ * append: a row of head_dim values (a query head, or K or V of a KV head) is
+ * HD / 8 lanes of eight values, so that every load and store is 16 bytes a lane
+ * and the row's largest magnitude, for int8, is a DPP reduction.  Rotation is
+ * the framework's: fl(fl(x0 c) - fl(x1 s)), fl(fl(x0 s) + fl(x1 c)).
+ *
+ * attention: see the kernels.
+ */
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "gq_paged.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+/* ------------------------------------------------------- append and read */
+struct AppendArgs {
+  PgdPages c;
+  PgdBatch b;
+  const void *q, *k, *v;
+  void *q_out;
+  const float *rope;
+  int n_heads, qs, qos, ks, vs, nq; /* nq: query rows a token, 0 without q */
+};
+
+/* maximum over a row's HD / 8 lanes */
+template <int HD>
+__device__ __forceinline__ float row_max(float m) {
+  m = fmaxf(m, gq_dpp<0x141>(m)); /* row_half_mirror: within 8 */
+  m = fmaxf(m, gq_dpp<0x4e>(m));
+  m = fmaxf(m, gq_dpp<0xb1>(m));
+  if (HD == 128) m = fmaxf(m, gq_dpp<0x140>(m)); /* row_mirror: the other eight */
+  return m;
+}
+
+/* round(y / d) to nearest even as if the quotient were exact: the candidate
+ * from the rounded one is off by one at most, and the sign of y - (c +- 1/2) d,
+ * which one fused operation gives exactly, says so. */
+__device__ __forceinline__ int quant(float y, float d) {
+  float c = __builtin_rintf(y / d);
+  const float up = __builtin_fmaf(-(c + 0.5f), d, y), dn = __builtin_fmaf(-(c - 0.5f), d, y);
+  const bool odd = ((int)c & 1) != 0;
+  if (up > 0.f || (up == 0.f && odd)) c += 1.f;
+  else if (dn < 0.f || (dn == 0.f && odd)) c -= 1.f;
+  return (int)fminf(fmaxf(c, -127.f), 127.f);
+}
+
+template <int CT, int XT, int HD>
+__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
+#pragma clang fp contract(off)
+  constexpr int LPR = HD / 8, RPW = GQ_WAVE / LPR; /* lanes a row, rows a wave */
+  const int lane = threadIdx.x & 63, sub = lane % LPR;
+  const int per = a.nq + 2 * a.c.n_kv; /* rows a token */
+  const long long w0 = ((long long)blockIdx.x * (kThreads / GQ_WAVE) + (threadIdx.x >> 6)) * RPW;
+  const long long total = (long long)a.b.n_tokens * per;
+  if (w0 >= total) return; /* uniform in the wave */
+  int s = pgd_seq_of(a.b, (int)(w0 / per));
+  const long long r = w0 + lane / LPR;
+  const int t = (int)(r / per), j = (int)(r % per);
+  if (r >= total) return;
+  /* a wave's rows are of one token, or of a few in a row */
+  if (a.b.first)
+    while (s < a.b.n_seqs && gld<int>(a.b.first + s + 1) <= t) s++;
+  else s = t;
+  if (s >= a.b.n_seqs) return;
+  const int r0 = a.b.first ? gld<int>(a.b.first + s) : t, p0 = gld<int>(a.b.pos + s);
+  if (t < r0 || p0 < 0) return;
+  const int p = p0 + (t - r0), page = pgd_page(a.c, a.b, s, p);
+  if (page < 0) return;
+  const bool isq = j < a.nq, isk = !isq && j < a.nq + a.c.n_kv;
+  const int h = isq ? j : isk ? j - a.nq : j - a.nq - a.c.n_kv;
+  float x[8];
+  if (isq) pgd_load8<XT>(a.q, (size_t)t * a.qs + (size_t)h * HD + 8 * sub, x);
+  else pgd_load8<XT>(isk ? a.k : a.v, (size_t)t * (isk ? a.ks : a.vs) + (size_t)h * HD + 8 * sub, x);
+  if (a.rope && (isq || isk)) {
+    const float *cs = a.rope + (size_t)p * HD + 8 * sub;
+    const float4 c0 = gld<float4>(cs), c1 = gld<float4>(cs + 4);
+    const float c[4] = {c0.x, c0.z, c1.x, c1.z}, n[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float e = x[2 * i], o = x[2 * i + 1];
+      x[2 * i] = e * c[i] - o * n[i];
+      x[2 * i + 1] = e * n[i] + o * c[i];
+    }
+  }
+  if (isq) {
+    pgd_store8<XT>(a.q_out, (size_t)t * a.qos + (size_t)h * HD + 8 * sub, x);
+    return;
+  }
+  const size_t row = pgd_row(a.c, page, h, p & ((1 << a.c.lg) - 1));
+  uint8_t *pool = isk ? a.c.k : a.c.v;
+  if constexpr (CT != GQ_I8_ROWS) {
+    pgd_store8<CT>(pool, row * HD + 8 * sub, x);
+  } else {
+    float m = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = fmaxf(m, __builtin_fabsf(x[i])), bad |= !(__builtin_fabsf(x[i]) < INFINITY);
+    m = row_max<HD>(bad ? INFINITY : m);
+    const bool lost = m == INFINITY;
+    const float d = lost ? __builtin_nanf("") : m / 127.0f;
+    int c[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = lost || !(d > 0.f) ? 0 : quant(x[i], d);
+    uint2 w;
+    w.x = (uint32_t)(c[0] & 255) | (uint32_t)(c[1] & 255) << 8 | (uint32_t)(c[2] & 255) << 16 | (uint32_t)c[3] << 24;
+    w.y = (uint32_t)(c[4] & 255) | (uint32_t)(c[5] & 255) << 8 | (uint32_t)(c[6] & 255) << 16 | (uint32_t)c[7] << 24;
+    gst<uint2>(pool + row * HD + 8 * sub, w);
+    if (sub == 0) gst<float>((isk ? a.c.ks : a.c.vs) + row, d);
+  }
+}
+
+struct ReadArgs {
+  PgdPages c;
+  PgdBatch b;
+  void *k, *v;
+  int ks, vs;
+};
+
+__device__ __forceinline__ float i8f(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+
+template <int CT, int XT, int HD>
+__global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
+  constexpr int LPR = HD / 8, RPW = GQ_WAVE / LPR;
+  const int lane = threadIdx.x & 63, sub = lane % LPR, per = 2 * a.c.n_kv;
+  const long long w0 = ((long long)blockIdx.x * (kThreads / GQ_WAVE) + (threadIdx.x >> 6)) * RPW;
+  const long long total = (long long)a.b.n_tokens * per;
+  if (w0 >= total) return;
+  int s = pgd_seq_of(a.b, (int)(w0 / per));
+  const long long r = w0 + lane / LPR;
+  const int t = (int)(r / per), j = (int)(r % per);
+  if (r >= total) return;
+  if (a.b.first)
+    while (s < a.b.n_seqs && gld<int>(a.b.first + s + 1) <= t) s++;
+  else s = t;
+  if (s >= a.b.n_seqs) return;
+  const int r0 = a.b.first ? gld<int>(a.b.first + s) : t, p0 = gld<int>(a.b.pos + s);
+  if (t < r0) return;
+  const int p = p0 + (t - r0), page = p0 < 0 ? -1 : pgd_page(a.c, a.b, s, p);
+  const bool isk = j < a.c.n_kv;
+  const int h = isk ? j : j - a.c.n_kv;
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (page >= 0) {
+    const size_t row = pgd_row(a.c, page, h, p & ((1 << a.c.lg) - 1));
+    const uint8_t *pool = isk ? a.c.k : a.c.v;
+    if constexpr (CT != GQ_I8_ROWS) {
+      pgd_load8<CT>(pool, row * HD + 8 * sub, x);
+    } else {
+      const uint2 w = gld<uint2>(pool + row * HD + 8 * sub);
+      const float d = gld<float>((isk ? a.c.ks : a.c.vs) + row);
+#pragma unroll
+      for (int i = 0; i < 4; i++) x[i] = i8f(w.x, i) * d, x[4 + i] = i8f(w.y, i) * d;
+    }
+  }
+  pgd_store8<XT>(isk ? a.k : a.v, (size_t)t * (isk ? a.ks : a.vs) + (size_t)h * HD + 8 * sub, x);
+}
+
+/* -------------------------------------------------------------- attention */
+struct AttArgs {
+  PgdPages c;
+  PgdBatch b;
+  const void *q;
+  void *out;
+  float *part_o, *part_ml; /* [row][head][nch][hd] and [..][2] */
+  int n_heads, G, qs, os;
+  int nch, chunk; /* parts of at most `chunk` keys, a multiple of 128 */
+  bool each;      /* every new token (blockIdx is a packed row), not the last of a sequence */
+  float scale;    /* log2(e) / sqrt(head_dim) */
+};
+
+/* x = hi + mid + lo exactly, bf16 each, for pairs */
+__device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+  hi = pgd_pack(x, y);
+  x -= pgd_lo(hi), y -= pgd_hi(hi);
+  mid = pgd_pack(x, y);
+  x -= pgd_lo(mid), y -= pgd_hi(mid);
+  lo = pgd_pack(x, y);
+}
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], gq_bf16x8 (&out)[N]) {
+  uint4 p[3];
+  split3(x[0], x[1], p[0].x, p[1].x, p[2].x);
+  split3(x[2], x[3], p[0].y, p[1].y, p[2].y);
+  split3(x[4], x[5], p[0].z, p[1].z, p[2].z);
+  split3(x[6], x[7], p[0].w, p[1].w, p[2].w);
+#pragma unroll
+  for (int i = 0; i < N; i++) out[i] = __builtin_bit_cast(gq_bf16x8, p[i]);
+}
+
+/* eight int8 codes as bf16, exactly */
+__device__ __forceinline__ gq_bf16x8 codes8(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(gq_bf16x8, make_uint4(pgd_pack(i8f(a, 0), i8f(a, 1)), pgd_pack(i8f(a, 2), i8f(a, 3)),
+                                                  pgd_pack(i8f(b, 0), i8f(b, 1)), pgd_pack(i8f(b, 2), i8f(b, 3))));
+}
+
+constexpr int kMaxG = 16;
+
+/* Attention of one query token (its G heads of KV head g) over the keys of one
+ * part, by four waves that take 32 (fp32 caches: 16) keys each in turn, every
+ * one with an online softmax of its own, joined through LDS at the end.  The
+ * matrix instructions do both products with the heads as columns:
+ *   S^T = K Q^T   A = K rows straight from memory: lane (c, j) = (lane % 16,
+ *                 lane / 16) holds key c, and the dims are dealt to the lane
+ *                 groups j so that each reads 16 bytes at a time; B = the
+ *                 queries, as exact sums of bf16 parts (three for fp32).  The
+ *                 lane gets head c's scores of keys 4 j + r, r < 4.
+ *   O^T += V^T P^T  B = the probabilities straight from that layout (in three
+ *                 bf16 parts for fp32 results, two for bf16 ones); A = V rows
+ *                 4 j + r, dims VD c .. VD c + VD - 1 as they lie in memory,
+ *                 transposed four by four within the lane (v_perm): tile t's
+ *                 row c is dim VD c + t.  The lane holds head c's outputs of
+ *                 dims VD (4 j + r) + t, so the softmax's rescale stays in the
+ *                 lane.
+ * int8 codes are exact in bf16; K's scale multiplies the score, V's the
+ * probability.  fp32 caches use the fp32 matrix instructions, which need no
+ * transposition (one key a step).  Keys that do not exist are masked, and V's
+ * rows there are zeroed: what stale memory holds cannot reach a sum. */
+template <int CT, int XT, int HD>
+__global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
+  constexpr int NW = kThreads / GQ_WAVE;
+  constexpr int TK = CT == GQ_F32 ? 1 : 2;   /* 16-key tiles a step */
+  constexpr int KL = HD * pgd_bytes(CT) / 64; /* 16-byte loads of a K row per lane */
+  constexpr int VD = HD / 16;                /* dims of a V row per lane */
+  constexpr int VW = VD * pgd_bytes(CT) / 4; /* dwords of them */
+  constexpr int NQ = XT == GQ_F32 ? 3 : 1, NP = XT == GQ_F32 ? 3 : 2;
+  __shared__ float sm[NW][kMaxG], sl[NW][kMaxG];
+  __shared__ float so[NW][kMaxG][HD + 4];
+  const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int bid = blockIdx.x;
+  const int g = bid % a.c.n_kv;
+  bid /= a.c.n_kv;
+  const int part = bid % a.nch, item = bid / a.nch;
+  /* sequence, row and length */
+  int s, row, len;
+  if (a.each) {
+    s = __builtin_amdgcn_readfirstlane(pgd_seq_of(a.b, item));
+    if (s >= a.b.n_seqs) return;
+    const int2 rn = pgd_rows(a.b, s);
+    row = item;
+    if (row < rn.x || row >= rn.x + rn.y) return;
+    const int p0 = gld<int>(a.b.pos + s);
+    len = p0 < 0 ? 0 : min(p0 + (row - rn.x) + 1, a.b.max_len);
+  } else {
+    s = item;
+    const int2 rn = pgd_rows(a.b, s);
+    if (rn.y < 1) return;
+    row = rn.x + rn.y - 1;
+    const int p0 = gld<int>(a.b.pos + s);
+    len = p0 < 0 ? 0 : min(p0 + rn.y, a.b.max_len);
+  }
+  const int parts = max(1, (len + a.chunk - 1) / a.chunk);
+  if (part >= parts) return;
+  const int k1 = min(len, (part + 1) * a.chunk);
+  const int ps = 1 << a.c.lg;
+
+  /* queries: head c of this KV head's group, zero past it */
+  const size_t qat = (size_t)row * a.qs + (size_t)(g * a.G + min(c, a.G - 1)) * HD;
+  constexpr int NS = CT == GQ_F32 ? HD / 16 : HD / 32; /* slices of 4 (fp32) or 8 dims per lane */
+  gq_bf16x8 qp[CT == GQ_F32 ? 1 : NS][NQ];
+  float qf[CT == GQ_F32 ? NS : 1][4];
+#pragma unroll
+  for (int i = 0; i < NS; i++) {
+    if constexpr (CT == GQ_F32) {
+      float x[8];
+      /* dims 16 i + 4 j .. + 3 */
+      const size_t at = qat + 16 * i + 4 * j;
+      if constexpr (XT == GQ_F32) {
+        const float4 u = gld<float4>((const float *)a.q + at);
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+      } else {
+        const uint2 u = gld<uint2>((const uint16_t *)a.q + at);
+        x[0] = pgd_lo(u.x), x[1] = pgd_hi(u.x), x[2] = pgd_lo(u.y), x[3] = pgd_hi(u.y);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) qf[i][e] = c < a.G ? x[e] : 0.f;
+    } else {
+      /* bf16: dims 32 i + 8 j .. + 7; int8: 64 (i / 2) + 16 j + 8 (i % 2) */
+      const int d = CT == GQ_BF16 ? 32 * i + 8 * j : 64 * (i >> 1) + 16 * j + 8 * (i & 1);
+      float x[8];
+      pgd_load8<XT>(a.q, qat + d, x);
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = c < a.G ? x[e] : 0.f;
+      split8<NQ>(x, qp[i]);
+    }
+  }
+
+  uint4 kr[TK][KL];
+  uint32_t vr[TK][4][VW];
+  float4 kd[TK], vd[TK];
+  int lim[TK];      /* keys of the tile that exist */
+  size_t base[TK];  /* its first row in the pool */
+  auto find = [&](int kb) {
+#pragma unroll
+    for (int u = 0; u < TK; u++) {
+      const int kt = kb + 16 * u;
+      const int page = __builtin_amdgcn_readfirstlane(kt < k1 ? pgd_page(a.c, a.b, s, kt) : -1);
+      lim[u] = page < 0 ? 0 : min(16, k1 - kt);
+      base[u] = pgd_row(a.c, max(page, 0), g, kt & (ps - 1));
+    }
+  };
+  auto loadk = [&]() {
+#pragma unroll
+    for (int u = 0; u < TK; u++) {
+      const uint8_t *kp = a.c.k + (base[u] + c) * (size_t)(HD * pgd_bytes(CT)) + 16 * j;
+#pragma unroll
+      for (int i = 0; i < KL; i++) kr[u][i] = gld_nt<uint4>(kp + 64 * i);
+      if constexpr (CT == GQ_I8_ROWS) kd[u] = gld<float4>(a.c.ks + base[u] + 4 * j);
+    }
+  };
+  auto loadv = [&]() {
+#pragma unroll
+    for (int u = 0; u < TK; u++) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint8_t *vp = a.c.v + (base[u] + 4 * j + r) * (size_t)(HD * pgd_bytes(CT)) + VW * 4 * c;
+        if constexpr (VW == 1) {
+          vr[u][r][0] = gld_nt<uint32_t>(vp);
+        } else if constexpr (VW == 2) {
+          const uint2 w = gld_nt<uint2>(vp);
+          vr[u][r][0] = w.x, vr[u][r][1] = w.y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < VW / 4; i++) {
+            const uint4 w = gld_nt<uint4>(vp + 16 * i);
+            vr[u][r][4 * i] = w.x, vr[u][r][4 * i + 1] = w.y, vr[u][r][4 * i + 2] = w.z, vr[u][r][4 * i + 3] = w.w;
+          }
+        }
+      }
+      if constexpr (CT == GQ_I8_ROWS) vd[u] = gld<float4>(a.c.vs + base[u] + 4 * j);
+    }
+  };
+
+  float m = -INFINITY, l = 0.f; /* l: this lane's keys only */
+  gq_f32x4 o[VD];
+#pragma unroll
+  for (int t = 0; t < VD; t++) o[t] = gq_f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int STEP = 16 * TK * NW;
+  for (int kb = part * a.chunk + 16 * TK * wave; kb < k1; kb += STEP) {
+    find(kb);
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < TK; u++) any |= lim[u] > 0;
+    if (!any) continue; /* uniform: the pages are the wave's */
+    loadk();
+    loadv();
+    float p[TK][4], mb = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < TK; u++) {
+      gq_f32x4 st = gq_f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (CT == GQ_F32) {
+        gq_f32x4 s1 = st;
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+          const float kf[4] = {__builtin_bit_cast(float, kr[u][i].x), __builtin_bit_cast(float, kr[u][i].y),
+                               __builtin_bit_cast(float, kr[u][i].z), __builtin_bit_cast(float, kr[u][i].w)};
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            st = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[i][e], st, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e + 1], qf[i][e + 1], s1, 0, 0, 0);
+          }
+        }
+        st += s1;
+      } else {
+#pragma unroll
+        for (int n = NQ - 1; n >= 0; n--)
+#pragma unroll
+          for (int i = 0; i < NS; i++) {
+            gq_bf16x8 kk;
+            if constexpr (CT == GQ_BF16) kk = __builtin_bit_cast(gq_bf16x8, kr[u][i]);
+            else if (i & 1) kk = codes8(kr[u][i >> 1].z, kr[u][i >> 1].w);
+            else kk = codes8(kr[u][i >> 1].x, kr[u][i >> 1].y);
+            st = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, qp[i][n], st, 0, 0, 0);
+          }
+      }
+      if constexpr (CT == GQ_I8_ROWS) st[0] *= kd[u].x, st[1] *= kd[u].y, st[2] *= kd[u].z, st[3] *= kd[u].w;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[u][r] = 4 * j + r < lim[u] ? st[r] * a.scale : -INFINITY;
+        mb = fmaxf(mb, p[u][r]);
+      }
+    }
+    mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
+    mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+    const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - ms);
+    m = mn;
+    float lb = 0.f;
+#pragma unroll
+    for (int u = 0; u < TK; u++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[u][r] = __builtin_amdgcn_exp2f(p[u][r] - ms);
+        lb += p[u][r];
+      }
+    l = __builtin_fmaf(l, alpha, lb);
+#pragma unroll
+    for (int t = 0; t < VD; t++) o[t] *= alpha;
+    /* rows that do not exist: their weight is 0, but 0 * NaN is not */
+#pragma unroll
+    for (int u = 0; u < TK; u++) {
+      if (lim[u] < 16) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const bool there = 4 * j + r < lim[u];
+#pragma unroll
+          for (int i = 0; i < VW; i++) vr[u][r][i] = there ? vr[u][r][i] : 0u;
+        }
+        if constexpr (CT == GQ_I8_ROWS) {
+          vd[u].x = 4 * j < lim[u] ? vd[u].x : 0.f, vd[u].y = 4 * j + 1 < lim[u] ? vd[u].y : 0.f;
+          vd[u].z = 4 * j + 2 < lim[u] ? vd[u].z : 0.f, vd[u].w = 4 * j + 3 < lim[u] ? vd[u].w : 0.f;
+        }
+      }
+    }
+    if constexpr (CT == GQ_F32) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int t = 0; t < VD; t++)
+          o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[0][r][t]), p[0][r], o[t], 0, 0, 0);
+    } else {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < TK; u++) {
+        if constexpr (CT == GQ_I8_ROWS) p[u][0] *= vd[u].x, p[u][1] *= vd[u].y, p[u][2] *= vd[u].z, p[u][3] *= vd[u].w;
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[4 * u + r] = p[u][r];
+      }
+      gq_bf16x8 pp[NP];
+      split8<NP>(x, pp);
+#pragma unroll
+      for (int t = 0; t < VD; t++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < TK; u++)
+#pragma unroll
+          for (int r = 0; r < 4; r += 2) {
+            if constexpr (CT == GQ_BF16)
+              w[2 * u + r / 2] = __builtin_amdgcn_perm(vr[u][r + 1][t / 2], vr[u][r][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
+            else
+              w[2 * u + r / 2] = pgd_pack(i8f(vr[u][r][t / 4], t & 3), i8f(vr[u][r + 1][t / 4], t & 3));
+          }
+        const gq_bf16x8 vv = __builtin_bit_cast(gq_bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+        for (int n = NP - 1; n >= 0; n--) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pp[n], o[t], 0, 0, 0);
+      }
+    }
+  }
+  /* the waves' results: head c, dims VD (4 j + r) + t */
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (j == 0) sm[wave][c] = m, sl[wave][c] = l;
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int t = 0; t < VD; t++) so[wave][c][VD * (4 * j + r) + t] = o[t][r];
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.G * HD; i += kThreads) {
+    const int h = i / HD, d = i % HD;
+    float M = sm[0][h];
+#pragma unroll
+    for (int w = 1; w < NW; w++) M = fmaxf(M, sm[w][h]);
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const float e = __builtin_amdgcn_exp2f(sm[w][h] - ms);
+      L = __builtin_fmaf(sl[w][h], e, L);
+      y = __builtin_fmaf(so[w][h][d], e, y);
+    }
+    const int qh = g * a.G + h;
+    if (parts == 1) {
+      y = L == 0.f ? 0.f : y / L; /* nothing seen: zeros */
+      const size_t at = (size_t)row * a.os + (size_t)qh * HD + d;
+      if constexpr (XT == GQ_F32) gst<float>((float *)a.out + at, y);
+      else gst<uint16_t>((uint16_t *)a.out + at, (uint16_t)pgd_pack(y, y));
+    } else {
+      const size_t at = ((size_t)item * a.n_heads + qh) * a.nch + part;
+      gst<float>(a.part_o + at * HD + d, y);
+      if (d == 0) gst<float>(a.part_ml + 2 * at, M), gst<float>(a.part_ml + 2 * at + 1, L);
+    }
+  }
+}
+
+/* ------------------------------------------------------------ entry points */
+struct DeviceGuard { /* the context's device is current for the call */
+  int prev = -1;
+  explicit DeviceGuard(int dev) {
+    int cur = -1;
+    if (hipGetDevice(&cur) == hipSuccess && cur != dev && hipSetDevice(dev) == hipSuccess) prev = cur;
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
+bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+/* 0, or -1 / -5 with the message set */
+int check_cache(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype) {
+  if (!c) return -1;
+  if (!p || !b) return gq_ctx_fail(c, -1, "paged: NULL pages or batch");
+  if (p->dtype != GQ_F32 && p->dtype != GQ_BF16 && p->dtype != GQ_I8_ROWS) return gq_ctx_fail(c, -1, "paged: cache dtype");
+  if (xtype != GQ_F32 && xtype != GQ_BF16) return gq_ctx_fail(c, -1, "paged: xtype is GQ_F32 or GQ_BF16");
+  if (!p->k || !p->v || !aligned(p->k) || !aligned(p->v)) return gq_ctx_fail(c, -1, "paged: K and V pools are not there, or not 16-byte aligned");
+  if (p->dtype == GQ_I8_ROWS && (!p->k_scale || !p->v_scale || !aligned(p->k_scale) || !aligned(p->v_scale)))
+    return gq_ctx_fail(c, -1, "paged: an int8 cache needs its scales, 16-byte aligned");
+  if (p->head_dim != 64 && p->head_dim != 128) return gq_ctx_fail(c, -1, "paged: head_dim is 64 or 128");
+  if (p->n_kv_heads < 1 || p->n_pages < 1) return gq_ctx_fail(c, -1, "paged: no KV heads or no pages");
+  if (p->page_size < 16 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+    return gq_ctx_fail(c, -1, "paged: page_size is a power of two from 16 to 1024");
+  if (b->n_seqs < 0 || b->n_tokens < 0) return gq_ctx_fail(c, -1, "paged: negative size of the batch");
+  if (b->n_seqs && (!b->table || !b->pos || b->table_stride < 1 || b->max_len < 0)) return gq_ctx_fail(c, -1, "paged: incomplete batch");
+  if (!b->first && b->n_tokens < b->n_seqs) return gq_ctx_fail(c, -1, "paged: fewer rows than sequences");
+  if (b->n_seqs && (long long)b->max_len > (long long)b->table_stride * p->page_size)
+    return gq_ctx_fail(c, -5, "paged: max_len passes the page table");
+  return 0;
+}
+/* rows of `width` values at a stride */
+bool row_ok(const void *p, int stride, long long width) { return p && aligned(p) && stride >= width && stride % 8 == 0; }
+
+PgdPages pages_of(const gq_pages *p) {
+  return PgdPages{(uint8_t *)p->k, (uint8_t *)p->v, p->k_scale, p->v_scale, p->n_pages, __builtin_ctz((unsigned)p->page_size), p->n_kv_heads};
+}
+PgdBatch batch_of(const gq_batch *b) {
+  return PgdBatch{b->table, b->pos, b->first, b->n_seqs, b->table_stride, b->n_tokens, b->max_len};
+}
+
+/* f<CT, XT, HD>() of run-time types */
+template <class F>
+void dispatch(int ct, int xt, int hd, F f) {
+  auto h = [&](auto CT, auto XT) {
+    if (hd == 64) f(CT, XT, std::integral_constant<int, 64>{});
+    else f(CT, XT, std::integral_constant<int, 128>{});
+  };
+  auto x = [&](auto CT) {
+    if (xt == GQ_F32) h(CT, std::integral_constant<int, GQ_F32>{});
+    else h(CT, std::integral_constant<int, GQ_BF16>{});
+  };
+  if (ct == GQ_F32) x(std::integral_constant<int, GQ_F32>{});
+  else if (ct == GQ_BF16) x(std::integral_constant<int, GQ_BF16>{});
+  else x(std::integral_constant<int, GQ_I8_ROWS>{});
+}
+
+/* workgroups of one-row-a-lane-group kernels; 0: more than a grid holds */
+unsigned row_blocks(long long rows, int hd) {
+  const long long per = kThreads / (hd / 8), n = (rows + per - 1) / per;
+  return n < (1ll << 31) ? (unsigned)n : 0u;
+}
+
+int attention(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads, const void *q, int q_stride,
+              void *out, int out_stride, bool each) {
+  if (int rc = check_cache(c, p, b, xtype)) return rc;
+  if (n_heads < 1 || n_heads % p->n_kv_heads || n_heads / p->n_kv_heads > kMaxG)
+    return gq_ctx_fail(c, -1, "paged attention: 1 to 16 query heads per KV head");
+  if (!b->n_seqs || !b->n_tokens) return 0;
+  const long long width = (long long)n_heads * p->head_dim;
+  if (!row_ok(q, q_stride, width) || !row_ok(out, out_stride, width))
+    return gq_ctx_fail(c, -1, "paged attention: rows of q and out (16-byte aligned, strides of 8 elements and no overlap)");
+  const GqCtxInfo ci = gq_ctx_info(c);
+  DeviceGuard guard(ci.dev);
+  AttArgs a{};
+  a.c = pages_of(p), a.b = batch_of(b), a.q = q, a.out = out, a.n_heads = n_heads, a.G = n_heads / p->n_kv_heads;
+  a.qs = q_stride, a.os = out_stride, a.each = each, a.scale = (float)(1.4426950408889634 / std::sqrt((double)p->head_dim));
+  a.nch = 1, a.chunk = (b->max_len + 127) / 128 * 128 + 128;
+  const long long blocks = (long long)(each ? b->n_tokens : b->n_seqs) * p->n_kv_heads * a.nch;
+  if (blocks >= (1ll << 31)) return gq_ctx_fail(c, -1, "paged attention: the batch passes a launch");
+  dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
+    hipLaunchKernelGGL((decode_kernel<CT(), XT(), HD()>), dim3((unsigned)blocks), dim3(kThreads), 0, ci.stream, a);
+  });
+  return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged attention launch");
+}
+
+} // namespace
+
+extern "C" int gq_hip_paged_append_dev(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads,
+                                       const void *q, int q_stride, void *q_out, int q_out_stride, const void *k,
+                                       int k_stride, const void *v, int v_stride, const float *rope, int n_rope) {
+  if (int rc = check_cache(c, p, b, xtype)) return rc;
+  if (q && n_heads < 1) return gq_ctx_fail(c, -1, "paged append: n_heads");
+  if (!b->n_seqs || !b->n_tokens) return 0;
+  const long long kvw = (long long)p->n_kv_heads * p->head_dim, qw = (long long)n_heads * p->head_dim;
+  if (!row_ok(k, k_stride, kvw) || !row_ok(v, v_stride, kvw) ||
+      (q && (!row_ok(q, q_stride, qw) || !row_ok(q_out, q_out_stride, qw))))
+    return gq_ctx_fail(c, -1, "paged append: rows of q, k and v (16-byte aligned, strides of 8 elements and no overlap)");
+  if (rope && !aligned(rope)) return gq_ctx_fail(c, -1, "paged append: rope is not 16-byte aligned");
+  if (rope && n_rope < b->max_len) return gq_ctx_fail(c, -5, "paged append: max_len passes the rope table");
+  const GqCtxInfo ci = gq_ctx_info(c);
+  DeviceGuard guard(ci.dev);
+  AppendArgs a{pages_of(p), batch_of(b), q, k, v, q_out, rope, n_heads, q_stride, q_out_stride, k_stride, v_stride, q ? n_heads : 0};
+  const unsigned blocks = row_blocks((long long)b->n_tokens * (a.nq + 2 * p->n_kv_heads), p->head_dim);
+  if (!blocks) return gq_ctx_fail(c, -1, "paged append: the batch passes a launch");
+  dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
+    hipLaunchKernelGGL((append_kernel<CT(), XT(), HD()>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
+  });
+  return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged append launch");
+}
+
+extern "C" int gq_hip_paged_read_dev(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, void *k, int k_stride,
+                                     void *v, int v_stride) {
+  if (int rc = check_cache(c, p, b, xtype)) return rc;
+  if (!b->n_seqs || !b->n_tokens) return 0;
+  const long long kvw = (long long)p->n_kv_heads * p->head_dim;
+  if (!row_ok(k, k_stride, kvw) || !row_ok(v, v_stride, kvw))
+    return gq_ctx_fail(c, -1, "paged read: rows of k and v (16-byte aligned, strides of 8 elements and no overlap)");
+  const GqCtxInfo ci = gq_ctx_info(c);
+  DeviceGuard guard(ci.dev);
+  ReadArgs a{pages_of(p), batch_of(b), k, v, k_stride, v_stride};
+  const unsigned blocks = row_blocks((long long)b->n_tokens * 2 * p->n_kv_heads, p->head_dim);
+  if (!blocks) return gq_ctx_fail(c, -1, "paged read: the batch passes a launch");
+  dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
+    hipLaunchKernelGGL((read_kernel<CT(), XT(), HD()>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
+  });
+  return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged read launch");
+}
+
+extern "C" int gq_hip_paged_decode_dev(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads,
+                                       const void *q, int q_stride, void *out, int out_stride) {
+  return attention(c, p, b, xtype, n_heads, q, q_stride, out, out_stride, false);
+}
+
+extern "C" int gq_hip_paged_prompt_dev(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads,
+                                       const void *q, int q_stride, void *out, int out_stride) {
+  return attention(c, p, b, xtype, n_heads, q, q_stride, out, out_stride, true);
+}

@@ -121,6 +121,8 @@ struct gq_ctx {
   void *stage[2] = {nullptr, nullptr};
   hipEvent_t stage_ev[2] = {nullptr, nullptr};
   SampleWs sw;
+  void *paged_ws = nullptr; /* gq_ctx_paged_ws */
+  size_t paged_cap = 0;
   /* pinned host memory: the token that a step, a prompt or a sampler picked
    * and the results a caller asked for (written by the argmax's or sampler's
    * launches, read after the wait), and a prompt's tokens (read by the
@@ -2210,6 +2212,20 @@ extern "C" int gq_hip_copy_dev(gq_ctx *c, void *dst, const void *src, size_t byt
   weights_written(c, dst, bytes);
   const int rc = gq_launch_copy(dst, src, bytes, c->n_cu, c->stream);
   return rc ? fail(c, rc, "copy: sizes and pointers must be multiples of 16 bytes") : 0;
+}
+
+/* ---- for the other translation units (gq_internal.h) ---- */
+GqCtxInfo gq_ctx_info(const gq_ctx *c) { return GqCtxInfo{c->dev, c->n_cu, c->stream}; }
+
+int gq_ctx_fail(gq_ctx *c, int code, const char *msg) { return fail(c, code, "%s", msg); }
+
+void *gq_ctx_paged_ws(gq_ctx *c, size_t bytes) {
+  if (c->paged_cap >= bytes) return c->paged_ws;
+  if (c->paged_ws) gq_hip_free(c, c->paged_ws); /* waits for the launches that still use it */
+  c->paged_cap = 0;
+  c->paged_ws = dev_alloc(c, bytes);
+  if (c->paged_ws) c->paged_cap = bytes;
+  return c->paged_ws;
 }
 
 extern "C" int gq_hip_silu_mul_dev(gq_ctx *c, float *gate, const float *up, int n) {

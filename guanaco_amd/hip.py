@@ -102,6 +102,11 @@ def _load():
                                                  _vp]),
         "gq_hip_prefill_attention_dev": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp,
                                                    _vp, _vp]),
+        "gq_hip_paged_append_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int,
+                                              _vp, C.c_int, _vp, C.c_int]),
+        "gq_hip_paged_read_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int]),
+        "gq_hip_paged_decode_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int]),
+        "gq_hip_paged_prompt_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int]),
         "gq_hip_chat_turn": (C.c_int, [_vp, C.POINTER(C.c_int32), C.c_int, C.POINTER(C.c_int), C.c_int, C.c_int,
                                           C.c_float, C.c_int, C.c_float, C.POINTER(C.c_int), C.POINTER(C.c_int32)]),
         "gq_hip_prefill": (C.c_int, [_vp, C.POINTER(C.c_int32), C.c_int, C.c_int, _fp, _fp,
@@ -155,6 +160,26 @@ class GqModel(C.Structure):
                                       "head_dim", "vocab")] + [
         ("rope_theta", C.c_float), ("rms_eps", C.c_float), ("layers", C.POINTER(GqLayer)),
         ("embed", GqWeight), ("lm_head", GqWeight), ("rms_final", _vp)]
+
+
+# element types of the paged cache and its rows, beside spec.F32
+BF16, I8_ROWS = 0x200, 0x201
+
+
+class GqPages(C.Structure):
+    """gq_pages: K and V pools of one layer (device pointers; k_scale and
+    v_scale with dtype I8_ROWS only)."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)] + [
+        (n, C.c_int) for n in ("dtype", "n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+
+class GqBatch(C.Structure):
+    """gq_batch: page table, positions before the new tokens and packed rows of
+    n_seqs sequences (device pointers; first None: one token each)."""
+
+    _fields_ = [("table", _vp), ("pos", _vp), ("first", _vp)] + [
+        (n, C.c_int) for n in ("n_seqs", "table_stride", "n_tokens", "max_len")]
 
 
 def mem_info(device_id=0):
@@ -355,6 +380,28 @@ class Context:
     def prefill_attention_dev(self, layer, pos, T, n_heads, q_buf, k_buf, v_buf, out_buf):
         return lib.gq_hip_prefill_attention_dev(self.h, layer, pos, T, n_heads, q_buf.ptr, k_buf.ptr,
                                                 v_buf.ptr, out_buf.ptr)
+
+    # ---- several sequences over a paged cache ----
+    def paged_append_dev(self, pages, batch, xtype, n_heads, q_buf, q_stride, q_out_buf, q_out_stride, k_buf, k_stride,
+                         v_buf, v_stride, rope_buf, n_rope):
+        """New tokens' rows into the cache; q_buf None: no queries, rope_buf
+        None: no rotation."""
+        p = lambda b: b.ptr if b is not None else None  # noqa: E731
+        self.check(lib.gq_hip_paged_append_dev(self.h, C.byref(pages), C.byref(batch), xtype, n_heads, p(q_buf), q_stride,
+                                               p(q_out_buf), q_out_stride, k_buf.ptr, k_stride, v_buf.ptr, v_stride,
+                                               p(rope_buf), n_rope), "paged_append")
+
+    def paged_read_dev(self, pages, batch, xtype, k_buf, k_stride, v_buf, v_stride):
+        self.check(lib.gq_hip_paged_read_dev(self.h, C.byref(pages), C.byref(batch), xtype, k_buf.ptr, k_stride, v_buf.ptr,
+                                             v_stride), "paged_read")
+
+    def paged_decode_dev(self, pages, batch, xtype, n_heads, q_buf, q_stride, out_buf, out_stride):
+        self.check(lib.gq_hip_paged_decode_dev(self.h, C.byref(pages), C.byref(batch), xtype, n_heads, q_buf.ptr, q_stride,
+                                               out_buf.ptr, out_stride), "paged_decode")
+
+    def paged_prompt_dev(self, pages, batch, xtype, n_heads, q_buf, q_stride, out_buf, out_stride):
+        self.check(lib.gq_hip_paged_prompt_dev(self.h, C.byref(pages), C.byref(batch), xtype, n_heads, q_buf.ptr, q_stride,
+                                               out_buf.ptr, out_stride), "paged_prompt")
 
     # ---- sessions ----
     def lctx_save(self, path, current_pos, tokens=None):

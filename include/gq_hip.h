@@ -406,6 +406,86 @@ int gq_hip_set_prefill_mode(gq_ctx *ctx, int mode);
 int gq_hip_set_prefill_copies(gq_ctx *ctx, int on);
 /* Bytes that they take on this context (0: there are none). */
 size_t gq_hip_prefill_copy_bytes(gq_ctx *ctx);
+/* ------------------------------------------------------- several sequences
+ * A paged K/V cache that many sequences share, and what runs over it: rows
+ * appended (rotated and quantised on the way) and read back, attention of one
+ * new token a sequence and of packed prompts, and sampling for a batch.  No
+ * counterpart in the reference, which holds one sequence in one fp32 slab.
+ *
+ * All pointers are device memory of the context's GPU, 16-byte aligned, and
+ * the caller's to keep (gq_hip_malloc, or any other allocation); calls are
+ * asynchronous on the context's stream and hold nothing of their arguments
+ * afterwards.  Lengths and pages are read on the device: a batch of the same
+ * n_seqs, n_tokens and max_len runs through the same launches whatever they
+ * say. */
+
+/* element types beside GQ_F32; none of the reference's DataType values */
+#define GQ_BF16 0x200
+#define GQ_I8_ROWS 0x201 /* int8 with one fp32 scale per row of head_dim values */
+
+/* K and V of one layer: n_pages pages of page_size positions (a power of two,
+ * 16 to 1024), each [n_kv_heads][page_size][head_dim] values of dtype (GQ_F32,
+ * GQ_BF16 or GQ_I8_ROWS).  GQ_I8_ROWS: a value is code * scale, the scales
+ * [n_pages][n_kv_heads][page_size]; NULL otherwise.  head_dim 64 or 128. */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int dtype, n_pages, page_size, n_kv_heads, head_dim;
+} gq_pages;
+
+/* Sequences and their new tokens.  Position p of sequence s lies in page
+ * table[s * table_stride + p / page_size]; an entry outside 0 .. n_pages - 1
+ * means that its positions do not exist.  pos[s] is the number of positions
+ * before the call's tokens (-1: an idle slot), first[s] the row of its first
+ * new token in the packed arrays of n_tokens rows, first[s + 1] - first[s]
+ * their number (0 is allowed).  first NULL: one token each, row s.  max_len: no
+ * sequence is longer, its new tokens included; positions from there on do not
+ * exist either.  It sizes launches and workspaces, so a close bound is faster. */
+typedef struct {
+  const int32_t *table, *pos, *first;
+  int n_seqs, table_stride, n_tokens, max_len;
+} gq_batch;
+
+/* New tokens' rows into the cache, steps 4 and 5 of transformer_layer
+ * (engine.c:372-392) for a batch: q (n_heads x head_dim a row) and k
+ * (n_kv_heads x head_dim) rotated by row pos[s] + t of rope, [n_rope][head_dim
+ * / 2] (cos, sin) pairs, as gq_hip_rope_append_dev rotates them (products and
+ * their sum rounded to fp32 one by one); rotated q to q_out (may be q), k and v
+ * to their page.  rope NULL: no rotation.  q NULL: no queries.
+ * xtype: GQ_F32 or GQ_BF16, of q, q_out, k and v.  Strides in elements between
+ * rows, multiples of 8.  GQ_BF16 caches round to nearest even; GQ_I8_ROWS takes
+ * scale = max |value| / 127 in fp32 and code = value / scale, rounded to
+ * nearest even as if exact, within -127 .. 127; a row that holds an infinity or
+ * NaN gets the scale NaN.  Tokens whose position does not exist are left out,
+ * and their q_out rows left as they were.
+ * 0; -1 bad argument; -5 max_len beyond the table's or rope's rows. */
+int gq_hip_paged_append_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
+                            const void *q, int q_stride, void *q_out, int q_out_stride, const void *k, int k_stride,
+                            const void *v, int v_stride, const float *rope, int n_rope);
+/* The rows of the batch's tokens (positions pos[s] + t) out of the cache: k and
+ * v, n_kv_heads x head_dim values of xtype a row, code * scale in fp32 and then
+ * rounded to nearest even.  pos 0 and first from whole lengths reads whole
+ * sequences, to save or to move them.  Positions that do not exist read as
+ * zeros; rows of no sequence stay as they were. */
+int gq_hip_paged_read_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, void *k, int k_stride,
+                          void *v, int v_stride);
+/* Attention of the last new token of each sequence (engine.c:433-509 for a
+ * batch): q row first[s + 1] - 1 (row s with first NULL) over positions 0 ..
+ * pos[s] + n - 1 of its cache, scaled by 1 / sqrt(head_dim), into the same row
+ * of out.  q and out: n_heads x head_dim values of xtype a row; n_heads /
+ * n_kv_heads from 1 to 16.  Scores, softmax and sums are fp32 throughout.  A
+ * token that sees no position gets zeros; rows of no sequence stay as they
+ * were.  Workspace for split sequences is the context's. */
+int gq_hip_paged_decode_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
+                            const void *q, int q_stride, void *out, int out_stride);
+/* The same for every new token: causal attention of packed prompts, token t of
+ * sequence s over positions 0 .. pos[s] + t, whose rows are in the cache.
+ * GQ_F32 queries keep fp32 accuracy throughout; with GQ_BF16 ones the
+ * probabilities are rounded to bf16 before they meet V, and a GQ_F32 cache's
+ * values before they meet either. */
+int gq_hip_paged_prompt_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
+                            const void *q, int q_stride, void *out, int out_stride);
+
 /* Device-to-device copy by a plain streaming kernel (bytes and both pointers
  * multiples of 16), asynchronous.  No reference counterpart: the known-size
  * workload that scales the HBM byte counters of the profiles. */
