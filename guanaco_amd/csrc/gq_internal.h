@@ -16,6 +16,17 @@ struct GqCtxInfo {
   hipStream_t stream;
 };
 GqCtxInfo gq_ctx_info(const gq_ctx *c);
+/* the context's device is current until the end of the scope */
+struct GqDeviceGuard {
+  int prev = -1;
+  explicit GqDeviceGuard(int dev) {
+    int cur = -1;
+    if (hipGetDevice(&cur) == hipSuccess && cur != dev && hipSetDevice(dev) == hipSuccess) prev = cur;
+  }
+  ~GqDeviceGuard() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
 /* sets the context's error message and returns code */
 int gq_ctx_fail(gq_ctx *c, int code, const char *msg);
 /* the context's workspace of the paged entry points, at least so many bytes;

@@ -489,17 +489,6 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
 }
 
 /* ------------------------------------------------------------ entry points */
-struct DeviceGuard { /* the context's device is current for the call */
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    int cur = -1;
-    if (hipGetDevice(&cur) == hipSuccess && cur != dev && hipSetDevice(dev) == hipSuccess) prev = cur;
-  }
-  ~DeviceGuard() {
-    if (prev >= 0) (void)hipSetDevice(prev);
-  }
-};
-
 bool aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 /* 0, or -1 / -5 with the message set */
@@ -564,7 +553,7 @@ int attention(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_
   if (!row_ok(q, q_stride, width) || !row_ok(out, out_stride, width))
     return gq_ctx_fail(c, -1, "paged attention: rows of q and out (16-byte aligned, strides of 8 elements and no overlap)");
   const GqCtxInfo ci = gq_ctx_info(c);
-  DeviceGuard guard(ci.dev);
+  GqDeviceGuard guard(ci.dev);
   AttArgs a{};
   a.c = pages_of(p), a.b = batch_of(b), a.q = q, a.out = out, a.n_heads = n_heads, a.G = n_heads / p->n_kv_heads;
   a.qs = q_stride, a.os = out_stride, a.each = each, a.scale = (float)(1.4426950408889634 / std::sqrt((double)p->head_dim));
@@ -592,7 +581,7 @@ extern "C" int gq_hip_paged_append_dev(gq_ctx *c, const gq_pages *p, const gq_ba
   if (rope && !aligned(rope)) return gq_ctx_fail(c, -1, "paged append: rope is not 16-byte aligned");
   if (rope && n_rope < b->max_len) return gq_ctx_fail(c, -5, "paged append: max_len passes the rope table");
   const GqCtxInfo ci = gq_ctx_info(c);
-  DeviceGuard guard(ci.dev);
+  GqDeviceGuard guard(ci.dev);
   AppendArgs a{pages_of(p), batch_of(b), q, k, v, q_out, rope, n_heads, q_stride, q_out_stride, k_stride, v_stride, q ? n_heads : 0};
   const unsigned blocks = row_blocks((long long)b->n_tokens * (a.nq + 2 * p->n_kv_heads), p->head_dim);
   if (!blocks) return gq_ctx_fail(c, -1, "paged append: the batch passes a launch");
@@ -610,7 +599,7 @@ extern "C" int gq_hip_paged_read_dev(gq_ctx *c, const gq_pages *p, const gq_batc
   if (!row_ok(k, k_stride, kvw) || !row_ok(v, v_stride, kvw))
     return gq_ctx_fail(c, -1, "paged read: rows of k and v (16-byte aligned, strides of 8 elements and no overlap)");
   const GqCtxInfo ci = gq_ctx_info(c);
-  DeviceGuard guard(ci.dev);
+  GqDeviceGuard guard(ci.dev);
   ReadArgs a{pages_of(p), batch_of(b), k, v, k_stride, v_stride};
   const unsigned blocks = row_blocks((long long)b->n_tokens * 2 * p->n_kv_heads, p->head_dim);
   if (!blocks) return gq_ctx_fail(c, -1, "paged read: the batch passes a launch");

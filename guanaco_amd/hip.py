@@ -107,6 +107,7 @@ def _load():
         "gq_hip_paged_read_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, _vp, C.c_int, _vp, C.c_int]),
         "gq_hip_paged_decode_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int]),
         "gq_hip_paged_prompt_dev": (C.c_int, [_vp, _vp, _vp, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int]),
+        "gq_hip_sample_rows_dev": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
         "gq_hip_chat_turn": (C.c_int, [_vp, C.POINTER(C.c_int32), C.c_int, C.POINTER(C.c_int), C.c_int, C.c_int,
                                           C.c_float, C.c_int, C.c_float, C.POINTER(C.c_int), C.POINTER(C.c_int32)]),
         "gq_hip_prefill": (C.c_int, [_vp, C.POINTER(C.c_int32), C.c_int, C.c_int, _fp, _fp,
@@ -402,6 +403,15 @@ class Context:
     def paged_prompt_dev(self, pages, batch, xtype, n_heads, q_buf, q_stride, out_buf, out_stride):
         self.check(lib.gq_hip_paged_prompt_dev(self.h, C.byref(pages), C.byref(batch), xtype, n_heads, q_buf.ptr, q_stride,
                                                out_buf.ptr, out_stride), "paged_prompt")
+
+    def sample_rows_dev(self, logits_buf, rows, vocab, row_stride, temperature_buf, top_k_buf, top_p_buf, min_p_buf, rnd_buf,
+                        tokens_buf, logprobs_buf=None):
+        """The next token of every row; a parameter's buffer None: its filter
+        is off (temperature 1)."""
+        p = lambda b: b.ptr if b is not None else None  # noqa: E731
+        self.check(lib.gq_hip_sample_rows_dev(self.h, logits_buf.ptr, rows, vocab, row_stride, p(temperature_buf), p(top_k_buf),
+                                              p(top_p_buf), p(min_p_buf), rnd_buf.ptr, tokens_buf.ptr, p(logprobs_buf)),
+                   "sample_rows")
 
     # ---- sessions ----
     def lctx_save(self, path, current_pos, tokens=None):

@@ -486,6 +486,30 @@ int gq_hip_paged_decode_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *
 int gq_hip_paged_prompt_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
                             const void *q, int q_stride, void *out, int out_stride);
 
+/* The next token of every row of a batch, from random numbers given: logits
+ * [rows][row_stride], vocab of them a row (at most 2^20), and per row, all in
+ * device memory (4-byte aligned):
+ *   temperature  w_i = e^((x_i - max x) / temperature); not above 0: the
+ *                largest logit's token (lowest index).  NULL: 1
+ *   top_k        only the k largest logits, the lowest indexes among equal
+ *                ones; 0 or less, or NULL: all
+ *   top_p        of those in descending order (equal ones by index) the
+ *                shortest run whose w sum to top_p of theirs, at least the
+ *                first; 1 or more, or NULL: all
+ *   min_p        of those the ones with w_i >= min_p (above 1 counts as 1);
+ *                0 or less, or NULL: all
+ *   rnd          in [0, 1): the first token in index order at which the sum of
+ *                the kept w passes rnd times their whole sum
+ * to tokens[rows], and log(w / whole sum) to logprobs[rows] (may be NULL; 0
+ * for temperature 0).  The weights and sums are exact to 2^-45 of the largest
+ * and the same in every call.  NaN and -infinity are never picked; a row of
+ * nothing else gets -1 and -infinity.  Asynchronous on the context's stream.
+ * gq_hip_sample_dev follows the reference's samplers for one row instead:
+ * another order of the sums, one of the filters, and libc's rand(). */
+int gq_hip_sample_rows_dev(gq_ctx *ctx, const float *logits, int rows, int vocab, int row_stride,
+                           const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                           const float *rnd, int32_t *tokens, float *logprobs);
+
 /* Device-to-device copy by a plain streaming kernel (bytes and both pointers
  * multiples of 16), asynchronous.  No reference counterpart: the known-size
  * workload that scales the HBM byte counters of the profiles. */

@@ -1,4 +1,5 @@
-"""The host side of the paged entry points on a CPU: gq_paged.hip linked with
+"""The host side of the paged entry points and of the batch sampler on a CPU:
+gq_paged.hip and gq_sample_rows.hip linked with
 tests/native/fake_paged.cpp, which stands for the HIP runtime and the context
 and counts launches.  What is refused launches nothing; what is taken runs on
 the context's device and leaves the caller's current."""
@@ -37,7 +38,8 @@ def build(d, *sources):
 def lib(tmp_path_factory):
     if not os.path.exists(HIPCC):
         pytest.skip("no hipcc")
-    src = [os.path.join(ROOT, "guanaco_amd", "csrc", "gq_paged.hip"), os.path.join(ROOT, "tests", "native", "fake_paged.cpp")]
+    src = [os.path.join(ROOT, "guanaco_amd", "csrc", n) for n in ("gq_paged.hip", "gq_sample_rows.hip")]
+    src.append(os.path.join(ROOT, "tests", "native", "fake_paged.cpp"))
     lib = C.CDLL(build(tmp_path_factory.mktemp("fake_paged"), *src))
     for n in (n for n in H.EXPORTS if hasattr(lib, n)):
         f, g = getattr(lib, n), getattr(H.lib, n)
@@ -151,3 +153,30 @@ def test_nothing_to_do_launches_nothing(lib, call):
     assert call(lib, b=batch(n_seqs=0, table=None, pos=None)) == 0
     assert call(lib, b=batch(n_tokens=0)) == 0
     assert lib.fake_launches() == 0
+
+
+def sample(lib, logits=A, rows=4, vocab=1000, stride=1000, t=A, k=A, p=A, m=A, rnd=A, tokens=A, logprobs=A):
+    return lib.gq_hip_sample_rows_dev(lib.fake_ctx(), logits, rows, vocab, stride, t, k, p, m, rnd, tokens, logprobs)
+
+
+@pytest.mark.parametrize("what", [dict(), dict(t=None, k=None, p=None, m=None, logprobs=None), dict(vocab=1 << 20, stride=1 << 20),
+                                  dict(vocab=1, stride=7), dict(logits=A + 4, rnd=A + 8)])
+def test_sampling_taken(lib, what):
+    lib.fake_reset(0)
+    lib.fake_set_device(2)
+    assert sample(lib, **what) == 0 and lib.fake_launches() >= 1 and lib.fake_device() == 2
+
+
+@pytest.mark.parametrize("what", [dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 20) + 1, stride=1 << 21), dict(stride=999),
+                                  dict(logits=None), dict(rnd=None), dict(tokens=None), dict(logits=A + 2), dict(k=A + 1),
+                                  dict(logprobs=A + 3)])
+def test_sampling_refused(lib, what):
+    lib.fake_reset(0)
+    assert sample(lib, **what) == -1
+    assert lib.fake_launches() == 0 and lib.fake_error()
+    assert lib.gq_hip_sample_rows_dev(None, A, 1, 10, 10, A, A, A, A, A, A, A) == -1
+
+
+def test_sampling_of_no_rows(lib):
+    lib.fake_reset(0)
+    assert sample(lib, rows=0, logits=None) == 0 and lib.fake_launches() == 0
