@@ -39,11 +39,11 @@ __device__ __forceinline__ int pgd_seq_of(const PgdBatch &b, int t) {
   return b.n_seqs;
 }
 
-/* (row of the first new token, their number); none where the rows are not in
- * the packed arrays */
+/* (row of the first new token, their number) of a sequence, s uniform in the
+ * wave; none where the rows are not in the packed arrays */
 __device__ __forceinline__ int2 pgd_rows(const PgdBatch &b, int s) {
   if (!b.first) return make_int2(s, s < b.n_tokens ? 1 : 0);
-  const int r0 = gld<int>(b.first + s), r1 = gld<int>(b.first + s + 1);
+  const int r0 = gq_sld<int>(b.first + s), r1 = gq_sld<int>(b.first + s + 1);
   return r0 < 0 || r1 > b.n_tokens || r1 <= r0 ? make_int2(0, 0) : make_int2(r0, r1 - r0);
 }
 
@@ -52,6 +52,13 @@ __device__ __forceinline__ int pgd_page(const PgdPages &c, const PgdBatch &b, in
   const int i = p >> c.lg;
   if (p < 0 || p >= b.max_len || i >= b.stride) return -1;
   const int page = gld<int>(b.table + (size_t)s * b.stride + i);
+  return (unsigned)page < (unsigned)c.n_pages ? page : -1;
+}
+/* The same through the scalar cache, s and p uniform in the wave. */
+__device__ __forceinline__ int pgd_page_u(const PgdPages &c, const PgdBatch &b, int s, int p) {
+  const int i = p >> c.lg;
+  if (p < 0 || p >= b.max_len || i >= b.stride) return -1;
+  const int page = gq_sld<int>(b.table + (size_t)s * b.stride + i);
   return (unsigned)page < (unsigned)c.n_pages ? page : -1;
 }
 /* row of (page, head, slot) in a pool */

@@ -51,68 +51,140 @@ __device__ __forceinline__ int quant(float y, float d) {
   return (int)fminf(fmaxf(c, -127.f), 127.f);
 }
 
-template <int CT, int XT, int HD>
+/* Where the rows of a wave are: U times RPW of the `per` rows of each packed
+ * token, one of them this lane's.  Rows are counted in tiles of 16 tokens, token
+ * after token for one head and then the next head: a wave's rows are neighbours
+ * in a page, their scales too. */
+constexpr int kRowTile = 16;
+template <int U>
+struct Rows {
+  int t[U], j[U];     /* token and which of its rows; t -1: none */
+  int p[U], page[U];  /* position and page, -1: it does not exist */
+};
+template <int U, int RPW>
+__device__ __forceinline__ bool find_rows(const PgdPages &c, const PgdBatch &b, int per, int sub_row, Rows<U> &o) {
+  static_assert(kRowTile % (U * RPW) == 0, "a wave's rows are of one head's tile");
+  const uint32_t w0 = (blockIdx.x * (uint32_t)(kThreads / GQ_WAVE) + (threadIdx.x >> 6)) * (uint32_t)(U * RPW);
+  const uint32_t t0 = w0 / (uint32_t)(kRowTile * per) * kRowTile;
+  if (t0 >= (uint32_t)b.n_tokens) return false; /* uniform in the wave */
+  const int s0 = pgd_seq_of(b, __builtin_amdgcn_readfirstlane((int)t0));
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const uint32_t r = w0 - t0 * per + u * RPW + sub_row;
+    const int t = (int)(t0 + r % kRowTile);
+    int s = s0;
+    o.j[u] = (int)(r / kRowTile);
+    if (t < b.n_tokens) {
+      if (!b.first) s = t;
+      else
+        while (s < b.n_seqs && gld<int>(b.first + s + 1) <= t) s++;
+    }
+    const bool in = t < b.n_tokens && s < b.n_seqs;
+    const int sc = in ? s : 0;
+    const int r0 = b.first ? gld<int>(b.first + sc) : t, p0 = gld<int>(b.pos + sc);
+    o.t[u] = in && t >= r0 ? t : -1;
+    o.p[u] = p0 < 0 ? -1 : p0 + (t - r0);
+    o.page[u] = o.t[u] < 0 || o.p[u] < 0 ? -1 : pgd_page(c, b, sc, o.p[u]);
+  }
+  return true;
+}
+
+/* A lane's eight values of a row: dims 8 sub .. + 7, or with SPLIT 4 sub .. + 3
+ * of either half, which makes every access of fp32 rows whole lines. */
+template <int T, bool SPLIT, int HD>
+__device__ __forceinline__ void load_row(const void *base, size_t at, int sub, float (&x)[8]) {
+  if constexpr (!SPLIT) {
+    pgd_load8<T>(base, at + 8 * sub, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const size_t p = at + i * (HD / 2) + 4 * sub;
+      if constexpr (T == GQ_F32) {
+        const float4 w = gld<float4>((const float *)base + p);
+        x[4 * i] = w.x, x[4 * i + 1] = w.y, x[4 * i + 2] = w.z, x[4 * i + 3] = w.w;
+      } else {
+        const uint2 w = gld<uint2>((const uint16_t *)base + p);
+        x[4 * i] = pgd_lo(w.x), x[4 * i + 1] = pgd_hi(w.x), x[4 * i + 2] = pgd_lo(w.y), x[4 * i + 3] = pgd_hi(w.y);
+      }
+    }
+  }
+}
+template <int T, bool SPLIT, int HD>
+__device__ __forceinline__ void store_row(void *base, size_t at, int sub, const float (&x)[8]) {
+  if constexpr (!SPLIT) {
+    pgd_store8<T>(base, at + 8 * sub, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const size_t p = at + i * (HD / 2) + 4 * sub;
+      if constexpr (T == GQ_F32) gst<float4>((float *)base + p, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+      else gst<uint2>((uint16_t *)base + p, make_uint2(pgd_pack(x[4 * i], x[4 * i + 1]), pgd_pack(x[4 * i + 2], x[4 * i + 3])));
+    }
+  }
+}
+
+template <int CT, int XT, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
 #pragma clang fp contract(off)
   constexpr int LPR = HD / 8, RPW = GQ_WAVE / LPR; /* lanes a row, rows a wave */
-  const int lane = threadIdx.x & 63, sub = lane % LPR;
-  const int per = a.nq + 2 * a.c.n_kv; /* rows a token */
-  const long long w0 = ((long long)blockIdx.x * (kThreads / GQ_WAVE) + (threadIdx.x >> 6)) * RPW;
-  const long long total = (long long)a.b.n_tokens * per;
-  if (w0 >= total) return; /* uniform in the wave */
-  int s = pgd_seq_of(a.b, (int)(w0 / per));
-  const long long r = w0 + lane / LPR;
-  const int t = (int)(r / per), j = (int)(r % per);
-  if (r >= total) return;
-  /* a wave's rows are of one token, or of a few in a row */
-  if (a.b.first)
-    while (s < a.b.n_seqs && gld<int>(a.b.first + s + 1) <= t) s++;
-  else s = t;
-  if (s >= a.b.n_seqs) return;
-  const int r0 = a.b.first ? gld<int>(a.b.first + s) : t, p0 = gld<int>(a.b.pos + s);
-  if (t < r0 || p0 < 0) return;
-  const int p = p0 + (t - r0), page = pgd_page(a.c, a.b, s, p);
-  if (page < 0) return;
-  const bool isq = j < a.nq, isk = !isq && j < a.nq + a.c.n_kv;
-  const int h = isq ? j : isk ? j - a.nq : j - a.nq - a.c.n_kv;
-  float x[8];
-  if (isq) pgd_load8<XT>(a.q, (size_t)t * a.qs + (size_t)h * HD + 8 * sub, x);
-  else pgd_load8<XT>(isk ? a.k : a.v, (size_t)t * (isk ? a.ks : a.vs) + (size_t)h * HD + 8 * sub, x);
-  if (a.rope && (isq || isk)) {
-    const float *cs = a.rope + (size_t)p * HD + 8 * sub;
-    const float4 c0 = gld<float4>(cs), c1 = gld<float4>(cs + 4);
-    const float c[4] = {c0.x, c0.z, c1.x, c1.z}, n[4] = {c0.y, c0.w, c1.y, c1.w};
+  constexpr int U = WIDE ? kRowTile / RPW : 1;
+  constexpr bool SPLIT = CT != GQ_BF16 || XT != GQ_BF16;
+  const int sub = threadIdx.x % LPR;
+  Rows<U> o;
+  if (!find_rows<U, RPW>(a.c, a.b, a.nq + 2 * a.c.n_kv, (threadIdx.x & 63) / LPR, o)) return;
+  float xs[U][8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float e = x[2 * i], o = x[2 * i + 1];
-      x[2 * i] = e * c[i] - o * n[i];
-      x[2 * i + 1] = e * n[i] + o * c[i];
+  for (int u = 0; u < U; u++) {
+    const int t = o.t[u], j = o.j[u];
+    if (t < 0) continue; /* the page may still be on its way */
+    if (j < a.nq) load_row<XT, SPLIT, HD>(a.q, (size_t)t * a.qs + (size_t)j * HD, sub, xs[u]);
+    else if (j < a.nq + a.c.n_kv) load_row<XT, SPLIT, HD>(a.k, (size_t)t * a.ks + (size_t)(j - a.nq) * HD, sub, xs[u]);
+    else load_row<XT, SPLIT, HD>(a.v, (size_t)t * a.vs + (size_t)(j - a.nq - a.c.n_kv) * HD, sub, xs[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    if (o.page[u] < 0) continue;
+    const int t = o.t[u], j = o.j[u], p = o.p[u];
+    const bool isq = j < a.nq, isk = !isq && j < a.nq + a.c.n_kv;
+    const int h = isq ? j : isk ? j - a.nq : j - a.nq - a.c.n_kv;
+    float(&x)[8] = xs[u];
+    if (a.rope && (isq || isk)) {
+      const float *cs = a.rope + (size_t)p * HD + (SPLIT ? 4 : 8) * sub;
+      const float4 c0 = gld<float4>(cs), c1 = gld<float4>(cs + (SPLIT ? HD / 2 : 4));
+      const float c[4] = {c0.x, c0.z, c1.x, c1.z}, n[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float e = x[2 * i], d = x[2 * i + 1];
+        x[2 * i] = e * c[i] - d * n[i];
+        x[2 * i + 1] = e * n[i] + d * c[i];
+      }
     }
-  }
-  if (isq) {
-    pgd_store8<XT>(a.q_out, (size_t)t * a.qos + (size_t)h * HD + 8 * sub, x);
-    return;
-  }
-  const size_t row = pgd_row(a.c, page, h, p & ((1 << a.c.lg) - 1));
-  uint8_t *pool = isk ? a.c.k : a.c.v;
-  if constexpr (CT != GQ_I8_ROWS) {
-    pgd_store8<CT>(pool, row * HD + 8 * sub, x);
-  } else {
-    float m = 0.f;
-    bool bad = false;
+    if (isq) {
+      store_row<XT, SPLIT, HD>(a.q_out, (size_t)t * a.qos + (size_t)h * HD, sub, x);
+      continue;
+    }
+    const size_t row = pgd_row(a.c, o.page[u], h, p & ((1 << a.c.lg) - 1));
+    uint8_t *pool = isk ? a.c.k : a.c.v;
+    if constexpr (CT != GQ_I8_ROWS) {
+      store_row<CT, SPLIT, HD>(pool, row * HD, sub, x);
+    } else {
+      float m = 0.f;
+      bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = fmaxf(m, __builtin_fabsf(x[i])), bad |= !(__builtin_fabsf(x[i]) < INFINITY);
-    m = row_max<HD>(bad ? INFINITY : m);
-    const bool lost = m == INFINITY;
-    const float d = lost ? __builtin_nanf("") : m / 127.0f;
-    int c[8];
+      for (int i = 0; i < 8; i++) m = fmaxf(m, __builtin_fabsf(x[i])), bad |= !(__builtin_fabsf(x[i]) < INFINITY);
+      m = row_max<HD>(bad ? INFINITY : m);
+      const bool lost = m == INFINITY;
+      const float d = lost ? __builtin_nanf("") : m / 127.0f;
+      int c[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) c[i] = lost || !(d > 0.f) ? 0 : quant(x[i], d);
-    uint2 w;
-    w.x = (uint32_t)(c[0] & 255) | (uint32_t)(c[1] & 255) << 8 | (uint32_t)(c[2] & 255) << 16 | (uint32_t)c[3] << 24;
-    w.y = (uint32_t)(c[4] & 255) | (uint32_t)(c[5] & 255) << 8 | (uint32_t)(c[6] & 255) << 16 | (uint32_t)c[7] << 24;
-    gst<uint2>(pool + row * HD + 8 * sub, w);
-    if (sub == 0) gst<float>((isk ? a.c.ks : a.c.vs) + row, d);
+      for (int i = 0; i < 8; i++) c[i] = lost || !(d > 0.f) ? 0 : quant(x[i], d);
+      uint2 w;
+      w.x = (uint32_t)(c[0] & 255) | (uint32_t)(c[1] & 255) << 8 | (uint32_t)(c[2] & 255) << 16 | (uint32_t)c[3] << 24;
+      w.y = (uint32_t)(c[4] & 255) | (uint32_t)(c[5] & 255) << 8 | (uint32_t)(c[6] & 255) << 16 | (uint32_t)c[7] << 24;
+      gst<uint32_t>(pool + row * HD + 4 * sub, w.x);
+      gst<uint32_t>(pool + row * HD + HD / 2 + 4 * sub, w.y);
+      if (sub == 0) gst<float>((isk ? a.c.ks : a.c.vs) + row, d);
+    }
   }
 }
 
@@ -125,40 +197,40 @@ struct ReadArgs {
 
 __device__ __forceinline__ float i8f(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 
-template <int CT, int XT, int HD>
+template <int CT, int XT, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
   constexpr int LPR = HD / 8, RPW = GQ_WAVE / LPR;
-  const int lane = threadIdx.x & 63, sub = lane % LPR, per = 2 * a.c.n_kv;
-  const long long w0 = ((long long)blockIdx.x * (kThreads / GQ_WAVE) + (threadIdx.x >> 6)) * RPW;
-  const long long total = (long long)a.b.n_tokens * per;
-  if (w0 >= total) return;
-  int s = pgd_seq_of(a.b, (int)(w0 / per));
-  const long long r = w0 + lane / LPR;
-  const int t = (int)(r / per), j = (int)(r % per);
-  if (r >= total) return;
-  if (a.b.first)
-    while (s < a.b.n_seqs && gld<int>(a.b.first + s + 1) <= t) s++;
-  else s = t;
-  if (s >= a.b.n_seqs) return;
-  const int r0 = a.b.first ? gld<int>(a.b.first + s) : t, p0 = gld<int>(a.b.pos + s);
-  if (t < r0) return;
-  const int p = p0 + (t - r0), page = p0 < 0 ? -1 : pgd_page(a.c, a.b, s, p);
-  const bool isk = j < a.c.n_kv;
-  const int h = isk ? j : j - a.c.n_kv;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (page >= 0) {
-    const size_t row = pgd_row(a.c, page, h, p & ((1 << a.c.lg) - 1));
+  constexpr int U = WIDE ? kRowTile / RPW : 1;
+  constexpr bool SPLIT = CT != GQ_BF16 || XT != GQ_BF16;
+  const int sub = threadIdx.x % LPR;
+  Rows<U> o;
+  if (!find_rows<U, RPW>(a.c, a.b, 2 * a.c.n_kv, (threadIdx.x & 63) / LPR, o)) return;
+  float x[U][8];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const bool isk = o.j[u] < a.c.n_kv;
+    if (o.page[u] < 0) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[u][i] = 0.f;
+      continue;
+    }
+    const size_t row = pgd_row(a.c, o.page[u], isk ? o.j[u] : o.j[u] - a.c.n_kv, o.p[u] & ((1 << a.c.lg) - 1));
     const uint8_t *pool = isk ? a.c.k : a.c.v;
     if constexpr (CT != GQ_I8_ROWS) {
-      pgd_load8<CT>(pool, row * HD + 8 * sub, x);
+      load_row<CT, SPLIT, HD>(pool, row * HD, sub, x[u]);
     } else {
-      const uint2 w = gld<uint2>(pool + row * HD + 8 * sub);
+      const uint2 w = make_uint2(gld<uint32_t>(pool + row * HD + 4 * sub), gld<uint32_t>(pool + row * HD + HD / 2 + 4 * sub));
       const float d = gld<float>((isk ? a.c.ks : a.c.vs) + row);
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[i] = i8f(w.x, i) * d, x[4 + i] = i8f(w.y, i) * d;
+      for (int i = 0; i < 4; i++) x[u][i] = i8f(w.x, i) * d, x[u][4 + i] = i8f(w.y, i) * d;
     }
   }
-  pgd_store8<XT>(isk ? a.k : a.v, (size_t)t * (isk ? a.ks : a.vs) + (size_t)h * HD + 8 * sub, x);
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    if (o.t[u] < 0) continue;
+    const bool isk = o.j[u] < a.c.n_kv;
+    store_row<XT, SPLIT, HD>(isk ? a.k : a.v, (size_t)o.t[u] * (isk ? a.ks : a.vs) + (size_t)(isk ? o.j[u] : o.j[u] - a.c.n_kv) * HD, sub, x[u]);
+  }
 }
 
 /* -------------------------------------------------------------- attention */
@@ -173,6 +245,17 @@ struct AttArgs {
   bool each;      /* every new token (blockIdx is a packed row), not the last of a sequence */
   float scale;    /* log2(e) / sqrt(head_dim) */
 };
+
+/* The row of sequence s's last new token and the positions it sees; false: no
+ * token. */
+__device__ __forceinline__ bool decode_row(const AttArgs &a, int s, int &row, int &len) {
+  const int2 rn = pgd_rows(a.b, s);
+  if (rn.y < 1) return false;
+  const int p0 = gq_sld<int>(a.b.pos + s);
+  row = rn.x + rn.y - 1;
+  len = p0 < 0 ? 0 : min(p0 + rn.y, a.b.max_len);
+  return true;
+}
 
 /* x = hi + mid + lo exactly, bf16 each, for pairs */
 __device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
@@ -249,11 +332,7 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
     len = p0 < 0 ? 0 : min(p0 + (row - rn.x) + 1, a.b.max_len);
   } else {
     s = item;
-    const int2 rn = pgd_rows(a.b, s);
-    if (rn.y < 1) return;
-    row = rn.x + rn.y - 1;
-    const int p0 = gld<int>(a.b.pos + s);
-    len = p0 < 0 ? 0 : min(p0 + rn.y, a.b.max_len);
+    if (!decode_row(a, s, row, len)) return;
   }
   const int parts = max(1, (len + a.chunk - 1) / a.chunk);
   if (part >= parts) return;
@@ -294,15 +373,14 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
   uint4 kr[TK][KL];
   uint32_t vr[TK][4][VW];
   float4 kd[TK], vd[TK];
-  int lim[TK];      /* keys of the tile that exist */
-  size_t base[TK];  /* its first row in the pool */
+  int lim[TK], nlim[TK]; /* keys of the tile that exist; of the next step's */
+  size_t base[TK];       /* the first row in the pool of the tile loaded last */
   auto find = [&](int kb) {
 #pragma unroll
     for (int u = 0; u < TK; u++) {
-      const int kt = kb + 16 * u;
-      const int page = __builtin_amdgcn_readfirstlane(kt < k1 ? pgd_page(a.c, a.b, s, kt) : -1);
-      lim[u] = page < 0 ? 0 : min(16, k1 - kt);
-      base[u] = pgd_row(a.c, max(page, 0), g, kt & (ps - 1));
+      const int kt = kb + 16 * u, page = kt < k1 ? pgd_page_u(a.c, a.b, s, kt) : -1;
+      nlim[u] = page < 0 ? 0 : min(16, k1 - kt);
+      base[u] = pgd_row(a.c, max(page, 0), g, kt & (ps - 1)); /* of none: any row there is, masked */
     }
   };
   auto loadk = [&]() {
@@ -342,14 +420,18 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
 #pragma unroll
   for (int t = 0; t < VD; t++) o[t] = gq_f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int STEP = 16 * TK * NW;
-  for (int kb = part * a.chunk + 16 * TK * wave; kb < k1; kb += STEP) {
-    find(kb);
-    bool any = false;
+  /* one set of registers: the next step's K loads once the scores have read K,
+   * its V once the products have read V */
+  const int kfirst = part * a.chunk + 16 * TK * wave;
+  if (kfirst < k1) find(kfirst), loadk(), loadv();
+  for (int kb = kfirst; kb < k1; kb += STEP) {
 #pragma unroll
-    for (int u = 0; u < TK; u++) any |= lim[u] > 0;
-    if (!any) continue; /* uniform: the pages are the wave's */
-    loadk();
-    loadv();
+    for (int u = 0; u < TK; u++) lim[u] = nlim[u];
+    const bool more = kb + STEP < k1;
+    if (more) find(kb + STEP);
+    float4 kdu[TK], vdu[TK];
+#pragma unroll
+    for (int u = 0; u < TK; u++) kdu[u] = kd[u], vdu[u] = vd[u];
     float p[TK][4], mb = -INFINITY;
 #pragma unroll
     for (int u = 0; u < TK; u++) {
@@ -379,13 +461,14 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
             st = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, qp[i][n], st, 0, 0, 0);
           }
       }
-      if constexpr (CT == GQ_I8_ROWS) st[0] *= kd[u].x, st[1] *= kd[u].y, st[2] *= kd[u].z, st[3] *= kd[u].w;
+      if constexpr (CT == GQ_I8_ROWS) st[0] *= kdu[u].x, st[1] *= kdu[u].y, st[2] *= kdu[u].z, st[3] *= kdu[u].w;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         p[u][r] = 4 * j + r < lim[u] ? st[r] * a.scale : -INFINITY;
         mb = fmaxf(mb, p[u][r]);
       }
     }
+    if (more) loadk();
     mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
     mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
     const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.f : mn;
@@ -413,8 +496,8 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
           for (int i = 0; i < VW; i++) vr[u][r][i] = there ? vr[u][r][i] : 0u;
         }
         if constexpr (CT == GQ_I8_ROWS) {
-          vd[u].x = 4 * j < lim[u] ? vd[u].x : 0.f, vd[u].y = 4 * j + 1 < lim[u] ? vd[u].y : 0.f;
-          vd[u].z = 4 * j + 2 < lim[u] ? vd[u].z : 0.f, vd[u].w = 4 * j + 3 < lim[u] ? vd[u].w : 0.f;
+          vdu[u].x = 4 * j < lim[u] ? vdu[u].x : 0.f, vdu[u].y = 4 * j + 1 < lim[u] ? vdu[u].y : 0.f;
+          vdu[u].z = 4 * j + 2 < lim[u] ? vdu[u].z : 0.f, vdu[u].w = 4 * j + 3 < lim[u] ? vdu[u].w : 0.f;
         }
       }
     }
@@ -428,7 +511,7 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
       float x[8];
 #pragma unroll
       for (int u = 0; u < TK; u++) {
-        if constexpr (CT == GQ_I8_ROWS) p[u][0] *= vd[u].x, p[u][1] *= vd[u].y, p[u][2] *= vd[u].z, p[u][3] *= vd[u].w;
+        if constexpr (CT == GQ_I8_ROWS) p[u][0] *= vdu[u].x, p[u][1] *= vdu[u].y, p[u][2] *= vdu[u].z, p[u][3] *= vdu[u].w;
 #pragma unroll
         for (int r = 0; r < 4; r++) x[4 * u + r] = p[u][r];
       }
@@ -451,6 +534,7 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
         for (int n = NP - 1; n >= 0; n--) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pp[n], o[t], 0, 0, 0);
       }
     }
+    if (more) loadv();
   }
   /* the waves' results: head c, dims VD (4 j + r) + t */
   l += __shfl_xor(l, 16, 64);
@@ -486,6 +570,71 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
       if (d == 0) gst<float>(a.part_ml + 2 * at, M), gst<float>(a.part_ml + 2 * at + 1, L);
     }
   }
+}
+
+/* The parts of a token's keys: out = sum_c o_c 2^(m_c - M) / sum_c l_c 2^(m_c -
+ * M), a workgroup per 32 dims of a head, eight lanes of four dims for each of
+ * 32 parts at a time. */
+template <int XT, int HD>
+__global__ __launch_bounds__(kThreads) void merge_kernel(AttArgs a) {
+  __shared__ float sacc[32][33], sL[32], sM[kThreads / GQ_WAVE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = tid & 7, cg = tid >> 3;
+  const int dg = blockIdx.x % (HD / 32), item = blockIdx.x / (HD / 32), s = item / a.n_heads, h = item % a.n_heads;
+  int row, len;
+  if (!decode_row(a, s, row, len)) return;
+  const int parts = (len + a.chunk - 1) / a.chunk;
+  if (parts <= 1) return; /* its one part has written the result */
+  const size_t at = (size_t)item * a.nch;
+  const float *ml = a.part_ml + 2 * at, *po = a.part_o + at * HD + 32 * dg + 4 * sub;
+  float M = -INFINITY;
+  for (int c = tid; c < parts; c += kThreads) M = fmaxf(M, gld<float>(ml + 2 * c));
+  M = gq_wave_max(M);
+  if (lane == 0) sM[wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3]));
+  const float ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = cg; c < parts; c += 32) {
+    const float2 e = gld<float2>(ml + 2 * c);
+    const float4 o = gld<float4>(po + (size_t)c * HD);
+    const float w = __builtin_amdgcn_exp2f(e.x - ms);
+    L = __builtin_fmaf(e.y, w, L);
+    y.x = __builtin_fmaf(o.x, w, y.x), y.y = __builtin_fmaf(o.y, w, y.y);
+    y.z = __builtin_fmaf(o.z, w, y.z), y.w = __builtin_fmaf(o.w, w, y.w);
+  }
+  if (sub == 0) sL[cg] = L;
+  sacc[cg][4 * sub] = y.x, sacc[cg][4 * sub + 1] = y.y, sacc[cg][4 * sub + 2] = y.z, sacc[cg][4 * sub + 3] = y.w;
+  __syncthreads();
+  if (tid < 32) {
+    float t = 0.f, l = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < 32; i++) t += sacc[i][tid], l += sL[i];
+    t = l == 0.f ? 0.f : t / l;
+    const size_t o = (size_t)row * a.os + (size_t)h * HD + 32 * dg + tid;
+    if constexpr (XT == GQ_F32) gst<float>((float *)a.out + o, t);
+    else gst<uint16_t>((uint16_t *)a.out + o, (uint16_t)pgd_pack(t, t));
+  }
+}
+
+/* Keys a part of a decode launch, a multiple of 128.  256 KB of K and V make a
+ * part long enough that its share of the merge does not show (64 sequences of
+ * up to 8192 positions, bf16, 8 KV heads: 187 us with 512 keys, 197 with 1024 and
+ * 209 where the rule stopped at 4096 parts; one of 131072, int8: 55 with 1024,
+ * 62 with 512, 96 with 256), shorter ones where they would leave less than two
+ * workgroups a CU (one sequence of 4096, bf16: 10.9 with 128 keys, 15.3 with
+ * 512).  One part, without the merge's launch of 3 us, where a sequence is
+ * short (one of 256, bf16: 6.6 against 9.3; of 512: 11.1 against 9.9), or where
+ * the sequences alone fill the chip (64 of 500: 20 against 32; 32 of 1000,
+ * int8: 19.6 against 21.8). */
+int decode_chunk(const gq_batch *b, const gq_pages *p, int n_cu) {
+  const int row = 2 * p->head_dim * pgd_bytes(p->dtype), by = 256 * 1024 / row;
+  const long long heads = (long long)b->n_seqs * p->n_kv_heads;
+  const int whole = std::max(1, (b->max_len + 127) / 128) * 128;
+  if (b->max_len <= std::min(384, 192 * 1024 / row) || (heads >= n_cu && b->max_len <= by)) return whole;
+  const long long even = (heads * b->max_len / (2 * n_cu) + 127) / 128 * 128;
+  return (int)std::min<long long>({(long long)by, std::max<long long>(even, 128), (long long)whole});
 }
 
 /* ------------------------------------------------------------ entry points */
@@ -537,10 +686,15 @@ void dispatch(int ct, int xt, int hd, F f) {
   else x(std::integral_constant<int, GQ_I8_ROWS>{});
 }
 
-/* workgroups of one-row-a-lane-group kernels; 0: more than a grid holds */
-unsigned row_blocks(long long rows, int hd) {
-  const long long per = kThreads / (hd / 8), n = (rows + per - 1) / per;
-  return n < (1ll << 31) ? (unsigned)n : 0u;
+/* A whole tile a wave (WIDE), its loads under way together, where that leaves
+ * two waves a SIMD; below, a load each and more waves.  8122 tokens of 48 rows
+ * with their read: 63 us against 72. */
+bool wide_rows(long long rows) { return rows >= 32768; }
+/* their workgroups; 0: more rows than they count */
+unsigned row_blocks(long long tokens, int each, int hd, bool wide) {
+  const long long rows = (tokens + kRowTile - 1) / kRowTile * kRowTile * each;
+  const long long per = wide ? kThreads / GQ_WAVE * kRowTile : kThreads / (hd / 8);
+  return rows < (1ll << 31) - per ? (unsigned)((rows + per - 1) / per) : 0u;
 }
 
 int attention(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads, const void *q, int q_stride,
@@ -558,10 +712,22 @@ int attention(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_
   a.c = pages_of(p), a.b = batch_of(b), a.q = q, a.out = out, a.n_heads = n_heads, a.G = n_heads / p->n_kv_heads;
   a.qs = q_stride, a.os = out_stride, a.each = each, a.scale = (float)(1.4426950408889634 / std::sqrt((double)p->head_dim));
   a.nch = 1, a.chunk = (b->max_len + 127) / 128 * 128 + 128;
+  if (!each) {
+    a.chunk = decode_chunk(b, p, ci.n_cu);
+    a.nch = std::max(1, (b->max_len + a.chunk - 1) / a.chunk);
+    if (a.nch > 1) {
+      const size_t rows = (size_t)b->n_seqs * n_heads * a.nch;
+      a.part_o = (float *)gq_ctx_paged_ws(c, sizeof(float) * rows * (p->head_dim + 2));
+      if (!a.part_o) return -4;
+      a.part_ml = a.part_o + rows * p->head_dim;
+    }
+  }
   const long long blocks = (long long)(each ? b->n_tokens : b->n_seqs) * p->n_kv_heads * a.nch;
-  if (blocks >= (1ll << 31)) return gq_ctx_fail(c, -1, "paged attention: the batch passes a launch");
+  if (blocks >= (1ll << 31) || (long long)b->n_seqs * n_heads * 4 >= (1ll << 31)) return gq_ctx_fail(c, -1, "paged attention: the batch passes a launch");
   dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
     hipLaunchKernelGGL((decode_kernel<CT(), XT(), HD()>), dim3((unsigned)blocks), dim3(kThreads), 0, ci.stream, a);
+    if (a.nch > 1)
+      hipLaunchKernelGGL((merge_kernel<XT(), HD()>), dim3((unsigned)(b->n_seqs * n_heads * (HD() / 32))), dim3(kThreads), 0, ci.stream, a);
   });
   return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged attention launch");
 }
@@ -583,10 +749,13 @@ extern "C" int gq_hip_paged_append_dev(gq_ctx *c, const gq_pages *p, const gq_ba
   const GqCtxInfo ci = gq_ctx_info(c);
   GqDeviceGuard guard(ci.dev);
   AppendArgs a{pages_of(p), batch_of(b), q, k, v, q_out, rope, n_heads, q_stride, q_out_stride, k_stride, v_stride, q ? n_heads : 0};
-  const unsigned blocks = row_blocks((long long)b->n_tokens * (a.nq + 2 * p->n_kv_heads), p->head_dim);
+  const int each = a.nq + 2 * p->n_kv_heads;
+  const bool wide = wide_rows((long long)b->n_tokens * each);
+  const unsigned blocks = row_blocks(b->n_tokens, each, p->head_dim, wide);
   if (!blocks) return gq_ctx_fail(c, -1, "paged append: the batch passes a launch");
   dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
-    hipLaunchKernelGGL((append_kernel<CT(), XT(), HD()>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
+    if (wide) hipLaunchKernelGGL((append_kernel<CT(), XT(), HD(), true>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
+    else hipLaunchKernelGGL((append_kernel<CT(), XT(), HD(), false>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
   });
   return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged append launch");
 }
@@ -601,10 +770,13 @@ extern "C" int gq_hip_paged_read_dev(gq_ctx *c, const gq_pages *p, const gq_batc
   const GqCtxInfo ci = gq_ctx_info(c);
   GqDeviceGuard guard(ci.dev);
   ReadArgs a{pages_of(p), batch_of(b), k, v, k_stride, v_stride};
-  const unsigned blocks = row_blocks((long long)b->n_tokens * 2 * p->n_kv_heads, p->head_dim);
+  const int each = 2 * p->n_kv_heads;
+  const bool wide = wide_rows((long long)b->n_tokens * each);
+  const unsigned blocks = row_blocks(b->n_tokens, each, p->head_dim, wide);
   if (!blocks) return gq_ctx_fail(c, -1, "paged read: the batch passes a launch");
   dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
-    hipLaunchKernelGGL((read_kernel<CT(), XT(), HD()>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
+    if (wide) hipLaunchKernelGGL((read_kernel<CT(), XT(), HD(), true>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
+    else hipLaunchKernelGGL((read_kernel<CT(), XT(), HD(), false>), dim3(blocks), dim3(kThreads), 0, ci.stream, a);
   });
   return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged read launch");
 }
