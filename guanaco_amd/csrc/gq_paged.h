@@ -1,6 +1,6 @@
 /*
  * gq_paged.h — what the kernels over the paged K/V cache share
- * (gq_paged.hip).
+ * (gq_paged.hip, gq_paged_prompt.hip).
  */
 #ifndef GQ_PAGED_H
 #define GQ_PAGED_H
@@ -95,5 +95,50 @@ __device__ __forceinline__ void pgd_store8(void *base, size_t at, const float (&
     gst<uint4>((uint16_t *)base + at, make_uint4(pgd_pack(x[0], x[1]), pgd_pack(x[2], x[3]), pgd_pack(x[4], x[5]), pgd_pack(x[6], x[7])));
   }
 }
+
+/* byte i of a dword as a signed integer */
+__device__ __forceinline__ float i8f(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+
+/* x = hi + mid + lo exactly, bf16 each, for pairs */
+__device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+  hi = pgd_pack(x, y);
+  x -= pgd_lo(hi), y -= pgd_hi(hi);
+  mid = pgd_pack(x, y);
+  x -= pgd_lo(mid), y -= pgd_hi(mid);
+  lo = pgd_pack(x, y);
+}
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], gq_bf16x8 (&out)[N]) {
+  uint4 p[3];
+  split3(x[0], x[1], p[0].x, p[1].x, p[2].x);
+  split3(x[2], x[3], p[0].y, p[1].y, p[2].y);
+  split3(x[4], x[5], p[0].z, p[1].z, p[2].z);
+  split3(x[6], x[7], p[0].w, p[1].w, p[2].w);
+#pragma unroll
+  for (int i = 0; i < N; i++) out[i] = __builtin_bit_cast(gq_bf16x8, p[i]);
+}
+
+/* eight int8 codes as bf16, exactly */
+__device__ __forceinline__ gq_bf16x8 codes8(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(gq_bf16x8, make_uint4(pgd_pack(i8f(a, 0), i8f(a, 1)), pgd_pack(i8f(a, 2), i8f(a, 3)),
+                                                  pgd_pack(i8f(b, 0), i8f(b, 1)), pgd_pack(i8f(b, 2), i8f(b, 3))));
+}
+
+constexpr int kMaxG = 16; /* query heads per KV head */
+
+/* attention of new tokens over the cache */
+struct AttArgs {
+  PgdPages c;
+  PgdBatch b;
+  const void *q;
+  void *out;
+  float *part_o, *part_ml; /* [row][head][nch][hd] and [..][2] */
+  int n_heads, G, qs, os;
+  int nch, chunk; /* decode: parts of at most `chunk` keys, a multiple of 128 */
+  float scale;    /* log2(e) / sqrt(head_dim) */
+};
+
+/* gq_paged_prompt.hip: every new token's attention; 0, or -4 */
+int gq_launch_paged_prompt(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu, hipStream_t s);
 
 #endif

@@ -195,7 +195,6 @@ struct ReadArgs {
   int ks, vs;
 };
 
-__device__ __forceinline__ float i8f(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 
 template <int CT, int XT, int HD, bool WIDE>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
@@ -234,18 +233,6 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
 }
 
 /* -------------------------------------------------------------- attention */
-struct AttArgs {
-  PgdPages c;
-  PgdBatch b;
-  const void *q;
-  void *out;
-  float *part_o, *part_ml; /* [row][head][nch][hd] and [..][2] */
-  int n_heads, G, qs, os;
-  int nch, chunk; /* parts of at most `chunk` keys, a multiple of 128 */
-  bool each;      /* every new token (blockIdx is a packed row), not the last of a sequence */
-  float scale;    /* log2(e) / sqrt(head_dim) */
-};
-
 /* The row of sequence s's last new token and the positions it sees; false: no
  * token. */
 __device__ __forceinline__ bool decode_row(const AttArgs &a, int s, int &row, int &len) {
@@ -257,32 +244,6 @@ __device__ __forceinline__ bool decode_row(const AttArgs &a, int s, int &row, in
   return true;
 }
 
-/* x = hi + mid + lo exactly, bf16 each, for pairs */
-__device__ __forceinline__ void split3(float x, float y, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
-  hi = pgd_pack(x, y);
-  x -= pgd_lo(hi), y -= pgd_hi(hi);
-  mid = pgd_pack(x, y);
-  x -= pgd_lo(mid), y -= pgd_hi(mid);
-  lo = pgd_pack(x, y);
-}
-template <int N>
-__device__ __forceinline__ void split8(const float (&x)[8], gq_bf16x8 (&out)[N]) {
-  uint4 p[3];
-  split3(x[0], x[1], p[0].x, p[1].x, p[2].x);
-  split3(x[2], x[3], p[0].y, p[1].y, p[2].y);
-  split3(x[4], x[5], p[0].z, p[1].z, p[2].z);
-  split3(x[6], x[7], p[0].w, p[1].w, p[2].w);
-#pragma unroll
-  for (int i = 0; i < N; i++) out[i] = __builtin_bit_cast(gq_bf16x8, p[i]);
-}
-
-/* eight int8 codes as bf16, exactly */
-__device__ __forceinline__ gq_bf16x8 codes8(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(gq_bf16x8, make_uint4(pgd_pack(i8f(a, 0), i8f(a, 1)), pgd_pack(i8f(a, 2), i8f(a, 3)),
-                                                  pgd_pack(i8f(b, 0), i8f(b, 1)), pgd_pack(i8f(b, 2), i8f(b, 3))));
-}
-
-constexpr int kMaxG = 16;
 
 /* Attention of one query token (its G heads of KV head g) over the keys of one
  * part, by four waves that take 32 (fp32 caches: 16) keys each in turn, every
@@ -321,19 +282,9 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
   bid /= a.c.n_kv;
   const int part = bid % a.nch, item = bid / a.nch;
   /* sequence, row and length */
-  int s, row, len;
-  if (a.each) {
-    s = __builtin_amdgcn_readfirstlane(pgd_seq_of(a.b, item));
-    if (s >= a.b.n_seqs) return;
-    const int2 rn = pgd_rows(a.b, s);
-    row = item;
-    if (row < rn.x || row >= rn.x + rn.y) return;
-    const int p0 = gld<int>(a.b.pos + s);
-    len = p0 < 0 ? 0 : min(p0 + (row - rn.x) + 1, a.b.max_len);
-  } else {
-    s = item;
-    if (!decode_row(a, s, row, len)) return;
-  }
+  const int s = item;
+  int row, len;
+  if (!decode_row(a, s, row, len)) return;
   const int parts = max(1, (len + a.chunk - 1) / a.chunk);
   if (part >= parts) return;
   const int k1 = min(len, (part + 1) * a.chunk);
@@ -420,15 +371,15 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
 #pragma unroll
   for (int t = 0; t < VD; t++) o[t] = gq_f32x4{0.f, 0.f, 0.f, 0.f};
   constexpr int STEP = 16 * TK * NW;
-  /* one set of registers: the next step's K loads once the scores have read K,
-   * its V once the products have read V */
-  const int kfirst = part * a.chunk + 16 * TK * wave;
-  if (kfirst < k1) find(kfirst), loadk(), loadv();
-  for (int kb = kfirst; kb < k1; kb += STEP) {
+  /* One set of registers: the next step's K loads once the scores have read K,
+   * its V once the products have read V.  The last step is one of its own:
+   * loads under a condition in the loop leave registers undefined behind it,
+   * and the compiler has then put other values over V still to be read. */
+  auto step = [&](int kb, auto MORE) {
+    constexpr bool more = decltype(MORE)::value;
 #pragma unroll
     for (int u = 0; u < TK; u++) lim[u] = nlim[u];
-    const bool more = kb + STEP < k1;
-    if (more) find(kb + STEP);
+    if constexpr (more) find(kb + STEP);
     float4 kdu[TK], vdu[TK];
 #pragma unroll
     for (int u = 0; u < TK; u++) kdu[u] = kd[u], vdu[u] = vd[u];
@@ -468,7 +419,7 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
         mb = fmaxf(mb, p[u][r]);
       }
     }
-    if (more) loadk();
+    if constexpr (more) loadk();
     mb = fmaxf(mb, __shfl_xor(mb, 16, 64));
     mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
     const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.f : mn;
@@ -534,7 +485,13 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
         for (int n = NP - 1; n >= 0; n--) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pp[n], o[t], 0, 0, 0);
       }
     }
-    if (more) loadv();
+    if constexpr (more) loadv();
+  };
+  int kb = part * a.chunk + 16 * TK * wave;
+  if (kb < k1) {
+    find(kb), loadk(), loadv();
+    for (; kb + STEP < k1; kb += STEP) step(kb, std::true_type{});
+    step(kb, std::false_type{});
   }
   /* the waves' results: head c, dims VD (4 j + r) + t */
   l += __shfl_xor(l, 16, 64);
@@ -697,39 +654,21 @@ unsigned row_blocks(long long tokens, int each, int hd, bool wide) {
   return rows < (1ll << 31) - per ? (unsigned)((rows + per - 1) / per) : 0u;
 }
 
-int attention(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads, const void *q, int q_stride,
-              void *out, int out_stride, bool each) {
+/* the arguments of an attention over the cache: 0, a status, or 1 for nothing
+ * to do */
+int att_args(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads, const void *q, int q_stride,
+             void *out, int out_stride, AttArgs &a) {
   if (int rc = check_cache(c, p, b, xtype)) return rc;
   if (n_heads < 1 || n_heads % p->n_kv_heads || n_heads / p->n_kv_heads > kMaxG)
     return gq_ctx_fail(c, -1, "paged attention: 1 to 16 query heads per KV head");
-  if (!b->n_seqs || !b->n_tokens) return 0;
+  if (!b->n_seqs || !b->n_tokens) return 1;
   const long long width = (long long)n_heads * p->head_dim;
   if (!row_ok(q, q_stride, width) || !row_ok(out, out_stride, width))
     return gq_ctx_fail(c, -1, "paged attention: rows of q and out (16-byte aligned, strides of 8 elements and no overlap)");
-  const GqCtxInfo ci = gq_ctx_info(c);
-  GqDeviceGuard guard(ci.dev);
-  AttArgs a{};
+  a = AttArgs{};
   a.c = pages_of(p), a.b = batch_of(b), a.q = q, a.out = out, a.n_heads = n_heads, a.G = n_heads / p->n_kv_heads;
-  a.qs = q_stride, a.os = out_stride, a.each = each, a.scale = (float)(1.4426950408889634 / std::sqrt((double)p->head_dim));
-  a.nch = 1, a.chunk = (b->max_len + 127) / 128 * 128 + 128;
-  if (!each) {
-    a.chunk = decode_chunk(b, p, ci.n_cu);
-    a.nch = std::max(1, (b->max_len + a.chunk - 1) / a.chunk);
-    if (a.nch > 1) {
-      const size_t rows = (size_t)b->n_seqs * n_heads * a.nch;
-      a.part_o = (float *)gq_ctx_paged_ws(c, sizeof(float) * rows * (p->head_dim + 2));
-      if (!a.part_o) return -4;
-      a.part_ml = a.part_o + rows * p->head_dim;
-    }
-  }
-  const long long blocks = (long long)(each ? b->n_tokens : b->n_seqs) * p->n_kv_heads * a.nch;
-  if (blocks >= (1ll << 31) || (long long)b->n_seqs * n_heads * 4 >= (1ll << 31)) return gq_ctx_fail(c, -1, "paged attention: the batch passes a launch");
-  dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
-    hipLaunchKernelGGL((decode_kernel<CT(), XT(), HD()>), dim3((unsigned)blocks), dim3(kThreads), 0, ci.stream, a);
-    if (a.nch > 1)
-      hipLaunchKernelGGL((merge_kernel<XT(), HD()>), dim3((unsigned)(b->n_seqs * n_heads * (HD() / 32))), dim3(kThreads), 0, ci.stream, a);
-  });
-  return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged attention launch");
+  a.qs = q_stride, a.os = out_stride, a.scale = (float)(1.4426950408889634 / std::sqrt((double)p->head_dim));
+  return 0;
 }
 
 } // namespace
@@ -783,10 +722,32 @@ extern "C" int gq_hip_paged_read_dev(gq_ctx *c, const gq_pages *p, const gq_batc
 
 extern "C" int gq_hip_paged_decode_dev(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads,
                                        const void *q, int q_stride, void *out, int out_stride) {
-  return attention(c, p, b, xtype, n_heads, q, q_stride, out, out_stride, false);
+  AttArgs a;
+  if (int rc = att_args(c, p, b, xtype, n_heads, q, q_stride, out, out_stride, a)) return rc > 0 ? 0 : rc;
+  const GqCtxInfo ci = gq_ctx_info(c);
+  GqDeviceGuard guard(ci.dev);
+  a.chunk = decode_chunk(b, p, ci.n_cu);
+  a.nch = std::max(1, (b->max_len + a.chunk - 1) / a.chunk);
+  const long long blocks = (long long)b->n_seqs * p->n_kv_heads * a.nch, rows = (long long)b->n_seqs * n_heads;
+  if (std::max(blocks, rows * (p->head_dim / 32)) >= (1ll << 31)) return gq_ctx_fail(c, -1, "paged decode: the batch passes a launch");
+  if (a.nch > 1) {
+    a.part_o = (float *)gq_ctx_paged_ws(c, sizeof(float) * rows * a.nch * (p->head_dim + 2));
+    if (!a.part_o) return -4;
+    a.part_ml = a.part_o + rows * a.nch * p->head_dim;
+  }
+  dispatch(p->dtype, xtype, p->head_dim, [&](auto CT, auto XT, auto HD) {
+    hipLaunchKernelGGL((decode_kernel<CT(), XT(), HD()>), dim3((unsigned)blocks), dim3(kThreads), 0, ci.stream, a);
+    if (a.nch > 1)
+      hipLaunchKernelGGL((merge_kernel<XT(), HD()>), dim3((unsigned)(rows * (HD() / 32))), dim3(kThreads), 0, ci.stream, a);
+  });
+  return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "paged decode launch");
 }
 
 extern "C" int gq_hip_paged_prompt_dev(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype, int n_heads,
                                        const void *q, int q_stride, void *out, int out_stride) {
-  return attention(c, p, b, xtype, n_heads, q, q_stride, out, out_stride, true);
+  AttArgs a;
+  if (int rc = att_args(c, p, b, xtype, n_heads, q, q_stride, out, out_stride, a)) return rc > 0 ? 0 : rc;
+  const GqCtxInfo ci = gq_ctx_info(c);
+  GqDeviceGuard guard(ci.dev);
+  return gq_launch_paged_prompt(a, p->dtype, xtype, p->head_dim, ci.n_cu, ci.stream) ? gq_ctx_fail(c, -4, "paged prompt launch") : 0;
 }

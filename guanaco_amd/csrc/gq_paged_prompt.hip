@@ -1,0 +1,415 @@
+/*
+ * gq_paged_prompt.hip — causal attention of packed prompts over the paged K/V
+ * cache on the bf16 matrix cores (gfx950).
+ */
+#include <algorithm>
+#include <type_traits>
+
+#include "gq_paged.h"
+
+namespace {
+
+typedef float gq_f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kPThreads = 512, kKeys = 64;
+
+/* The sequence and tile of a workgroup: tiles of tpt tokens, sequence after
+ * sequence; s = n_seqs past the last one. */
+__device__ __forceinline__ void find_tile(const PgdBatch &b, int tpt, int id, int &s, int &tile) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int s0 = 0; s0 < b.n_seqs; s0 += GQ_WAVE) {
+    const int q = s0 + lane, qc = min(q, b.n_seqs - 1);
+    int r0 = qc, r1 = qc + 1;
+    if (b.first) r0 = gld<int>(b.first + qc), r1 = gld<int>(b.first + qc + 1);
+    const bool in = q < b.n_seqs && r0 >= 0 && r1 <= b.n_tokens && r1 > r0;
+    int c = in ? (r1 - r0 + tpt - 1) / tpt : 0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(c, o, 64);
+      if (lane >= o) c += u;
+    }
+    const uint64_t hit = __ballot(before + c > id);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      s = s0 + l;
+      tile = id - before - (l ? __shfl(c, l - 1, 64) : 0);
+      return;
+    }
+    before += __shfl(c, 63, 64);
+  }
+  s = b.n_seqs, tile = 0;
+}
+
+/* Causal attention, flash-attention style.  A workgroup of eight waves takes 32
+ * RG query rows = floor(32 RG / G) tokens x the G query heads of KV head g, and
+ * streams their sequence's keys in blocks of 64: wave (rg, kh) rows 32 rg .. +
+ * 31, and with KH = 2 keys 32 kh .. + 31 of every block, the two halves joined
+ * at the end.
+ *   S^T = K Q^T    A = K [key][dim] from LDS, B = the queries, in registers
+ *                  for the whole kernel; lane (r, h) = (lane % 32, lane / 32)
+ *                  gets row r's scores of keys 8 a + 4 h + c (a, c < 4)
+ *   O^T += V^T P^T B = the probabilities straight from that layout: the 16
+ *                  keys of a step are taken in the order in which a lane holds
+ *                  them, and V lies in LDS as [dim][key] in the same order
+ *                  (four keys by four dims transposed in registers on the
+ *                  way); lane (r, h) holds row r's outputs, so the softmax's
+ *                  rescale and the division stay in the lane.
+ * The blocks are loaded a block ahead into registers, turned into bf16 and put
+ * into LDS, octets (16 bytes) XOR-swizzled by the row.  bf16 values and int8
+ * codes are exact there (the scales multiply scores and probabilities); fp32
+ * accuracy is kept by splitting an fp32 operand x into three bf16 numbers that
+ * sum to it, and keeping the partial products that are not below 2^-24: three
+ * for fp32 queries over a bf16 or int8 cache, six over an fp32 one.  bf16
+ * queries take bf16 probabilities, and round an fp32 cache's values to bf16.
+ *
+ * Keys that do not exist are zeros in LDS and masked, so that what stale
+ * memory holds cannot reach a sum. */
+template <int CT, int XT, int HD, int RG, int KH>
+__global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_kernel(AttArgs a) {
+  static_assert(RG * KH * GQ_WAVE == kPThreads, "eight waves");
+  constexpr int NX = XT == GQ_F32 ? 3 : 1, NK = NX == 3 && CT == GQ_F32 ? 3 : 1;
+  constexpr int NP = NX * NK == 9 ? 6 : NX; /* partial products */
+  /* their planes of K or V and of Q or P, the small ones first */
+  constexpr int kA[3][6] = {{0}, {0, 0, 0}, {1, 2, 0, 1, 0, 0}}, kB[3][6] = {{0}, {2, 1, 0}, {1, 0, 2, 0, 1, 0}};
+  constexpr int W = NP == 6 ? 2 : NP == 3 ? 1 : 0;
+  constexpr int NB = NK == 1 ? 2 : 1;        /* blocks in LDS */
+  constexpr int EB = pgd_bytes(CT);
+  constexpr int NO = HD / 8;                 /* octets of a K row */
+  constexpr int NSL = HD / 16, ND = HD / 32; /* dim slices of S^T, dim tiles of O^T */
+  constexpr int KT = 2 / KH;                 /* 32-key tiles of a wave's */
+  constexpr int KPL = kKeys * HD * 2;        /* bytes of one plane */
+  constexpr int KI = kKeys * NO / kPThreads; /* K octets a thread */
+  constexpr int KPP = kPThreads / NO;        /* keys a pass of them */
+  constexpr int VTH = 16 * HD / 4;           /* threads with four keys x four dims of V */
+  constexpr int NQ = NX == 3 ? 2 : 1;        /* planes of Q in registers; the third in LDS */
+  constexpr int QLO = NB * 2 * NK * KPL, SCL = QLO + (NX == 3 ? RG * NSL * 1024 : 0);
+  constexpr int LDS = SCL + (CT == GQ_I8_ROWS ? NB * 2 * kKeys * 4 : 0);
+  static_assert(KH == 1 || LDS >= RG * 64 * 4 * (ND * 16 + 2), "the halves' exchange fits");
+  __shared__ __attribute__((aligned(16))) uint8_t smem_[LDS];
+  __shared__ __attribute__((aligned(16))) int sok[NB][4]; /* whether the block's 16-key groups exist */
+  GQ_LDS uint8_t *smem = (GQ_LDS uint8_t *)smem_;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wv / KH, kh = wv % KH;
+  const int G = a.G, tpt = 32 * RG / G;
+  const int g = blockIdx.x % a.c.n_kv;
+  int s, tile;
+  find_tile(a.b, tpt, (int)(gridDim.x / a.c.n_kv - 1 - blockIdx.x / a.c.n_kv), s, tile);
+  s = __builtin_amdgcn_readfirstlane(s), tile = __builtin_amdgcn_readfirstlane(tile);
+  if (s >= a.b.n_seqs) return;
+  const int2 rn = pgd_rows(a.b, s);
+  const int p0 = gq_sld<int>(a.b.pos + s), t0 = tile * tpt, nt = min(tpt, rn.y - t0);
+  /* position that a row of the tile sees last; none of an idle sequence */
+  auto sees = [&](int row) { return p0 < 0 ? -1 : min(p0 + t0 + min(row / G, nt - 1), a.b.max_len - 1); };
+  const int pmax = sees(32 * RG - 1), nblk = (pmax + kKeys) / kKeys; /* 0 for -1 */
+  const int row = 32 * rg + r, tok = min(row / G, nt - 1), qh = g * G + row % G;
+  const bool live = row < tpt * G && row / G < nt;
+  const int cpos = sees(row), wlo = sees(32 * rg), whi = sees(32 * rg + 31);
+
+  /* this row's query: dims 16 i + 8 h .. + 7 */
+  gq_bf16x8 q[NSL][NQ];
+  const uint32_t qlo = (uint32_t)(QLO + (rg * 64 + lane) * 16);
+#pragma unroll
+  for (int i = 0; i < NSL; i++) {
+    float x[8];
+    pgd_load8<XT>(a.q, (size_t)(rn.x + t0 + tok) * a.qs + (size_t)qh * HD + 16 * i + 8 * h, x);
+    if constexpr (NX == 3) {
+      gq_bf16x8 p[3];
+      split8<3>(x, p);
+      q[i][0] = p[0], q[i][1] = p[1];
+      if (kh == 0) lst<gq_bf16x8>(smem, qlo + RG * 1024 * i, p[2]);
+    } else {
+      split8<1>(x, q[i]);
+    }
+  }
+
+  /* staging: K octet ko of keys kk, kk + KPP ..; V dims 4 vd .. + 3 of keys 4
+   * va .. + 3; a wave's keys are of one 16-key group each time */
+  const int ko = tid % NO, kk = tid / NO, vd = tid % (HD / 4), va = tid / (HD / 4);
+  const bool vtask = VTH == kPThreads || tid < VTH;
+  uint32_t kr[KI][2 * EB], vr[4][EB]; /* raw dwords */
+  float sc = 0.f;                     /* tid < 128: the scale of key tid % 64, K's then V's */
+  bool kok[KI], vok;                  /* the group's page is there */
+  int kpos[KI], vpos;
+  auto load = [&](int b) {
+    const int key0 = b * kKeys;
+    const int ps = (1 << a.c.lg) - 1;
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+      const int k = key0 + kk + KPP * i;
+      const int page = pgd_page_u(a.c, a.b, s, __builtin_amdgcn_readfirstlane(k & ~15));
+      kok[i] = page >= 0, kpos[i] = k;
+      const uint8_t *kp = a.c.k + (pgd_row(a.c, max(page, 0), g, k & ps) * HD + 8 * ko) * EB;
+      if constexpr (EB == 1) {
+        const uint2 w = gld<uint2>(kp);
+        kr[i][0] = w.x, kr[i][1] = w.y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < EB / 2; e++) {
+          const uint4 w = gld<uint4>(kp + 16 * e);
+          kr[i][4 * e] = w.x, kr[i][4 * e + 1] = w.y, kr[i][4 * e + 2] = w.z, kr[i][4 * e + 3] = w.w;
+        }
+      }
+    }
+    if (vtask) {
+      const int k = key0 + 4 * va;
+      const int page = pgd_page_u(a.c, a.b, s, __builtin_amdgcn_readfirstlane(k & ~15));
+      vok = page >= 0, vpos = k;
+      const uint8_t *vp = a.c.v + (pgd_row(a.c, max(page, 0), g, k & ps) * HD + 4 * vd) * EB;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if constexpr (EB == 1) {
+          vr[i][0] = gld<uint32_t>(vp + i * HD);
+        } else if constexpr (EB == 2) {
+          const uint2 w = gld<uint2>(vp + i * HD * 2);
+          vr[i][0] = w.x, vr[i][1] = w.y;
+        } else {
+          const uint4 w = gld<uint4>(vp + i * HD * 4);
+          vr[i][0] = w.x, vr[i][1] = w.y, vr[i][2] = w.z, vr[i][3] = w.w;
+        }
+      }
+    }
+    if constexpr (CT == GQ_I8_ROWS) {
+      if (tid < 2 * kKeys) {
+        const int k = key0 + tid % kKeys, page = pgd_page(a.c, a.b, s, k);
+        sc = page >= 0 && k <= pmax ? gld<float>((tid < kKeys ? a.c.ks : a.c.vs) + pgd_row(a.c, page, g, k & ps)) : 0.f;
+      }
+    }
+  };
+  auto stage = [&](int buf) {
+    const uint32_t kb = (uint32_t)(buf * 2 * NK * KPL), vb = kb + NK * KPL;
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+      const bool there = kok[i] && kpos[i] <= pmax;
+#pragma unroll
+      for (int e = 0; e < 2 * EB; e++) kr[i][e] = there ? kr[i][e] : 0u;
+      const int key = kk + KPP * i;
+      const uint32_t at = kb + (uint32_t)(key * HD * 2 + ((ko ^ (key & (NO - 1))) << 4));
+      if constexpr (CT == GQ_BF16) {
+        lst<uint4>(smem, at, make_uint4(kr[i][0], kr[i][1], kr[i][2], kr[i][3]));
+      } else if constexpr (CT == GQ_I8_ROWS) {
+        lst<gq_bf16x8>(smem, at, codes8(kr[i][0], kr[i][1]));
+      } else {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_bit_cast(float, kr[i][e]);
+        gq_bf16x8 p[NK];
+        split8<NK>(x, p);
+#pragma unroll
+        for (int n = 0; n < NK; n++) lst<gq_bf16x8>(smem, at + n * KPL, p[n]);
+      }
+    }
+    if (vtask) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < EB; e++) vr[i][e] = vok && vpos + i <= pmax ? vr[i][e] : 0u;
+      const int oct = 4 * (va >> 3) + 2 * (va >> 2 & 1) + (va & 1), half = va >> 1 & 1;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int dim = 4 * vd + j;
+        const uint32_t at = vb + (uint32_t)(dim * kKeys * 2 + ((oct ^ ((dim ^ (dim >> 3)) & 7)) << 4) + 8 * half);
+        if constexpr (CT == GQ_BF16) {
+          const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;
+          lst<uint2>(smem, at, make_uint2(__builtin_amdgcn_perm(vr[1][j / 2], vr[0][j / 2], sel),
+                                          __builtin_amdgcn_perm(vr[3][j / 2], vr[2][j / 2], sel)));
+        } else if constexpr (CT == GQ_I8_ROWS) {
+          lst<uint2>(smem, at, make_uint2(pgd_pack(i8f(vr[0][0], j), i8f(vr[1][0], j)), pgd_pack(i8f(vr[2][0], j), i8f(vr[3][0], j))));
+        } else {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[i] = __builtin_bit_cast(float, vr[i][j]);
+          uint2 p[3];
+          split3(x[0], x[1], p[0].x, p[1].x, p[2].x);
+          split3(x[2], x[3], p[0].y, p[1].y, p[2].y);
+#pragma unroll
+          for (int n = 0; n < NK; n++) lst<uint2>(smem, at + n * KPL, p[n]);
+        }
+      }
+      if ((va & 3) == 0 && vd == 0) sok[buf][va >> 2] = vok;
+    }
+    if constexpr (CT == GQ_I8_ROWS) {
+      if (tid < 2 * kKeys) lst<float>(smem, SCL + (buf * 2 * kKeys + tid) * 4, tid < kKeys ? sc * a.scale : sc);
+    }
+  };
+
+  float m = -INFINITY, l = 0.f; /* l: this lane's keys only */
+  gq_f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; d++) o[d] = gq_f32x16{};
+  /* operand addresses within a block: K row 32 kt + r, octet 2 i + h; V row 32 d
+   * + r, octet 4 kt + 2 t + h */
+  const uint32_t kbase = (uint32_t)((32 * kh + r) * HD * 2 + ((h ^ (r & (NO - 1))) << 4));
+  const uint32_t vbase = (uint32_t)(NK * KPL + r * kKeys * 2 + (((4 * kh + h) ^ ((r ^ (r >> 3)) & 7)) << 4));
+
+  auto compute = [&](int b, int buf) {
+    const int key0 = b * kKeys + 32 * kh;
+    if (key0 > whi) return; /* none of this wave's rows sees any (uniform) */
+    const uint32_t at = (uint32_t)(buf * 2 * NK * KPL);
+    gq_f32x16 st[KT];
+#pragma unroll
+    for (int t = 0; t < KT; t++) {
+      st[t] = gq_f32x16{};
+#pragma unroll
+      for (int i = 0; i < NSL; i++) {
+        gq_bf16x8 kv[NK], qv[NX];
+#pragma unroll
+        for (int n = 0; n < NK; n++) kv[n] = lld<gq_bf16x8>(smem, at + (kbase ^ (32 * i)) + 32 * t * HD * 2 + n * KPL);
+        qv[0] = q[i][0];
+        if constexpr (NX == 3) qv[1] = q[i][1], qv[2] = lld<gq_bf16x8>(smem, qlo + RG * 1024 * i);
+#pragma unroll
+        for (int u = 0; u < NP; u++) st[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kv[kA[W][u]], qv[kB[W][u]], st[t], 0, 0, 0);
+      }
+    }
+    const bool all = sok[buf][0] & sok[buf][1] & sok[buf][2] & sok[buf][3];
+    /* scores in units of log 2: key key0 + 32 t + 8 (e / 4) + 4 h + e % 4 */
+    float mb = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT; t++) {
+      if constexpr (CT == GQ_I8_ROWS) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 d = lld<float4>(smem, SCL + (buf * 2 * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
+          st[t][e] *= d.x, st[t][e + 1] *= d.y, st[t][e + 2] *= d.z, st[t][e + 3] *= d.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) st[t][e] *= a.scale;
+      }
+      if (!all || key0 + 32 * t + 31 > wlo) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int k = 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+          st[t][e] = key0 + k <= cpos && sok[buf][(32 * kh + k) >> 4] ? st[t][e] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) mb = fmaxf(mb, st[t][e]);
+    }
+    mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+    const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - ms);
+    m = mn;
+    l *= alpha;
+    gq_bf16x8 ps[2 * KT][NX];
+#pragma unroll
+    for (int t = 0; t < KT; t++) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        st[t][e] = __builtin_amdgcn_exp2f(st[t][e] - ms);
+        l += st[t][e];
+      }
+      if constexpr (CT == GQ_I8_ROWS) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 d = lld<float4>(smem, SCL + (buf * 2 * kKeys + kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
+          st[t][e] *= d.x, st[t][e + 1] *= d.y, st[t][e + 2] *= d.z, st[t][e + 3] *= d.w;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = st[t][8 * u + e];
+        split8<NX>(x, ps[2 * t + u]);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < ND; d++) {
+      gq_f32x16 pv = gq_f32x16{};
+#pragma unroll
+      for (int t = 0; t < 2 * KT; t++) {
+        gq_bf16x8 vv[NK];
+#pragma unroll
+        for (int n = 0; n < NK; n++)
+          vv[n] = lld<gq_bf16x8>(smem, at + (vbase ^ (((4 * d & 7) ^ (2 * t)) << 4)) + n * KPL + 32 * d * kKeys * 2);
+#pragma unroll
+        for (int u = 0; u < NP; u++) pv = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv[kA[W][u]], ps[t][kB[W][u]], pv, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[d][e] = __builtin_fmaf(o[d][e], alpha, pv[e]);
+    }
+  };
+
+  /* past the end the last block loads again: under a condition the loads would
+   * leave registers undefined (decode_kernel) */
+  if (nblk > 0) {
+    load(0);
+    if constexpr (NB == 2) {
+      stage(0);
+      load(min(1, nblk - 1));
+      __syncthreads();
+      for (int b = 0; b < nblk; b++) {
+        stage((b + 1) & 1); /* last read before the barrier below */
+        load(min(b + 2, nblk - 1));
+        compute(b, b & 1);
+        __syncthreads();
+      }
+    } else {
+      for (int b = 0; b < nblk; b++) {
+        __syncthreads(); /* the planes are free */
+        stage(0);
+        __syncthreads();
+        load(min(b + 1, nblk - 1));
+        compute(b, 0);
+      }
+      __syncthreads();
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (KH == 2) { /* kh = 1 hands (m, l, O) to kh = 0 */
+    GQ_LDS float *x = (GQ_LDS float *)smem + rg * 64 * (ND * 16 + 2);
+    if (kh == 1) {
+      x[lane] = m, x[64 + lane] = l;
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[64 * (2 + 16 * d + e) + lane] = o[d][e];
+    }
+    __syncthreads();
+    if (kh == 1) return;
+    const float m1 = x[lane], mt = fmaxf(m, m1), ms = mt == -INFINITY ? 0.f : mt;
+    const float s0 = __builtin_amdgcn_exp2f(m - ms), s1 = __builtin_amdgcn_exp2f(m1 - ms);
+    l = l * s0 + x[64 + lane] * s1;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[d][e] = o[d][e] * s0 + x[64 * (2 + 16 * d + e) + lane] * s1;
+  }
+  if (!live) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l; /* nothing seen: zeros */
+#pragma unroll
+  for (int d = 0; d < ND; d++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) { /* dims 32 d + 8 c + 4 h .. + 3 */
+      const size_t at = (size_t)(rn.x + t0 + tok) * a.os + (size_t)qh * HD + 32 * d + 8 * c + 4 * h;
+      const float y[4] = {o[d][4 * c] * inv, o[d][4 * c + 1] * inv, o[d][4 * c + 2] * inv, o[d][4 * c + 3] * inv};
+      if constexpr (XT == GQ_F32) gst<float4>((float *)a.out + at, make_float4(y[0], y[1], y[2], y[3]));
+      else gst<uint2>((uint16_t *)a.out + at, make_uint2(pgd_pack(y[0], y[1]), pgd_pack(y[2], y[3])));
+    }
+}
+
+template <int CT, int XT, int HD>
+int launch(const AttArgs &a, int n_cu, hipStream_t s) {
+  constexpr int RG = XT == GQ_F32 ? 4 : 8, KH = 8 / RG;
+  const int tpt = 32 * RG / a.G;
+  const long long tiles = a.b.n_tokens / tpt + std::min(a.b.n_seqs, a.b.n_tokens), blocks = tiles * a.c.n_kv;
+  if (blocks >= (1ll << 31)) return -4;
+  (void)n_cu;
+  hipLaunchKernelGGL((prompt_kernel<CT, XT, HD, RG, KH>), dim3((unsigned)blocks), dim3(kPThreads), 0, s, a);
+  return hipGetLastError() == hipSuccess ? 0 : -4;
+}
+
+template <int CT, int XT>
+int launch_hd(const AttArgs &a, int hd, int n_cu, hipStream_t s) {
+  return hd == 64 ? launch<CT, XT, 64>(a, n_cu, s) : launch<CT, XT, 128>(a, n_cu, s);
+}
+
+} // namespace
+
+int gq_launch_paged_prompt(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu, hipStream_t s) {
+  const bool f = xtype == GQ_F32;
+  if (cache == GQ_F32) return f ? launch_hd<GQ_F32, GQ_F32>(a, head_dim, n_cu, s) : launch_hd<GQ_F32, GQ_BF16>(a, head_dim, n_cu, s);
+  if (cache == GQ_BF16) return f ? launch_hd<GQ_BF16, GQ_F32>(a, head_dim, n_cu, s) : launch_hd<GQ_BF16, GQ_BF16>(a, head_dim, n_cu, s);
+  return f ? launch_hd<GQ_I8_ROWS, GQ_F32>(a, head_dim, n_cu, s) : launch_hd<GQ_I8_ROWS, GQ_BF16>(a, head_dim, n_cu, s);
+}

@@ -38,7 +38,7 @@ def build(d, *sources):
 def lib(tmp_path_factory):
     if not os.path.exists(HIPCC):
         pytest.skip("no hipcc")
-    src = [os.path.join(ROOT, "guanaco_amd", "csrc", n) for n in ("gq_paged.hip", "gq_sample_rows.hip")]
+    src = [os.path.join(ROOT, "guanaco_amd", "csrc", n) for n in ("gq_paged.hip", "gq_paged_prompt.hip", "gq_sample_rows.hip")]
     src.append(os.path.join(ROOT, "tests", "native", "fake_paged.cpp"))
     lib = C.CDLL(build(tmp_path_factory.mktemp("fake_paged"), *src))
     for n in (n for n in H.EXPORTS if hasattr(lib, n)):
