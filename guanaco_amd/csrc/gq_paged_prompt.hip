@@ -41,6 +41,19 @@ __device__ __forceinline__ void find_tile(const PgdBatch &b, int tpt, int id, in
   s = b.n_seqs, tile = 0;
 }
 
+/* the larger of a lane's value and that of the lane 32 away */
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, w[0]), __builtin_bit_cast(float, w[1]));
+}
+
+__device__ __forceinline__ void pin(gq_bf16x8 &v, float &f) {
+  uint4 w = __builtin_bit_cast(uint4, v);
+  asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w), "+v"(f));
+  v = __builtin_bit_cast(gq_bf16x8, w);
+}
+
 /* Causal attention, flash-attention style.  A workgroup of eight waves takes 32
  * RG query rows = floor(32 RG / G) tokens x the G query heads of KV head g, and
  * streams their sequence's keys in blocks of 64: wave (rg, kh) rows 32 rg .. +
@@ -74,6 +87,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   constexpr int kA[3][6] = {{0}, {0, 0, 0}, {1, 2, 0, 1, 0, 0}}, kB[3][6] = {{0}, {2, 1, 0}, {1, 0, 2, 0, 1, 0}};
   constexpr int W = NP == 6 ? 2 : NP == 3 ? 1 : 0;
   constexpr int NB = NK == 1 ? 2 : 1;        /* blocks in LDS */
+  constexpr bool PIPE = NX == 1;
   constexpr int EB = pgd_bytes(CT);
   constexpr int NO = HD / 8;                 /* octets of a K row */
   constexpr int NSL = HD / 16, ND = HD / 32; /* dim slices of S^T, dim tiles of O^T */
@@ -84,10 +98,9 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   constexpr int VTH = 16 * HD / 4;           /* threads with four keys x four dims of V */
   constexpr int NQ = NX == 3 ? 2 : 1;        /* planes of Q in registers; the third in LDS */
   constexpr int QLO = NB * 2 * NK * KPL, SCL = QLO + (NX == 3 ? RG * NSL * 1024 : 0);
-  constexpr int LDS = SCL + (CT == GQ_I8_ROWS ? NB * 2 * kKeys * 4 : 0);
+  constexpr int LDS = SCL + (CT == GQ_I8_ROWS ? (4 + NB) * kKeys * 4 : 0); /* scales: four blocks of K's, NB of V's */
   static_assert(KH == 1 || LDS >= RG * 64 * 4 * (ND * 16 + 2), "the halves' exchange fits");
   __shared__ __attribute__((aligned(16))) uint8_t smem_[LDS];
-  __shared__ __attribute__((aligned(16))) int sok[NB][4]; /* whether the block's 16-key groups exist */
   GQ_LDS uint8_t *smem = (GQ_LDS uint8_t *)smem_;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wv / KH, kh = wv % KH;
@@ -124,65 +137,91 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   }
 
   /* staging: K octet ko of keys kk, kk + KPP ..; V dims 4 vd .. + 3 of keys 4
-   * va .. + 3; a wave's keys are of one 16-key group each time */
+   * va .. + 3; a wave's keys are of one 16-key group each time, and so of one
+   * page. */
   const int ko = tid % NO, kk = tid / NO, vd = tid % (HD / 4), va = tid / (HD / 4);
   const bool vtask = VTH == kPThreads || tid < VTH;
   uint32_t kr[KI][2 * EB], vr[4][EB]; /* raw dwords */
   float sc = 0.f;                     /* tid < 128: the scale of key tid % 64, K's then V's */
-  bool kok[KI], vok;                  /* the group's page is there */
-  int kpos[KI], vpos;
-  auto load = [&](int b) {
-    const int key0 = b * kKeys;
-    const int ps = (1 << a.c.lg) - 1;
+  const int ps = (1 << a.c.lg) - 1;
+  uint32_t koff[KI]; /* within a page's rows for the head, from the block's first slot */
+#pragma unroll
+  for (int i = 0; i < KI; i++) koff[i] = (uint32_t)((((kk + KPP * i) & ps) * HD + 8 * ko) * EB);
+  const uint32_t voff = (uint32_t)((((4 * va) & ps) * HD + 4 * vd) * EB);
+  /* Pages of 64 groups of 16 keys at a time, lane i: group i of blocks 16 n .. 16
+   * n + 15, -1 where it does not exist; those of block b's 16 and the next 16. */
+  const int32_t *table = a.b.table + (size_t)s * a.b.stride;
+  auto lookup = [&](int n) {
+    const int p = 16 * (64 * n + lane), page = gld<int>(table + min(p >> a.c.lg, a.b.stride - 1));
+    return p <= pmax && (unsigned)page < (unsigned)a.c.n_pages ? page : -1;
+  };
+  int pg0 = -1, pg1 = -1, pgn = 0;
+  auto pages = [&](int b) { return (b >> 4) == pgn ? pg0 : pg1; };
+  auto exists = [&](int b) { return (int)(__ballot(pages(b) >= 0) >> (4 * (b & 15))) & 15; }; /* bit i: group i of b */
+  /* the row of block b's first slot in the page of a key's group (uniform) */
+  auto rows = [&](int b, int key) {
+    const int page = __builtin_amdgcn_readlane(pages(b), __builtin_amdgcn_readfirstlane(4 * (b & 15) + (key >> 4)));
+    return pgd_row(a.c, max(page, 0), g, (b * kKeys) & ps);
+  };
+  auto loadk = [&](int b) {
 #pragma unroll
     for (int i = 0; i < KI; i++) {
-      const int k = key0 + kk + KPP * i;
-      const int page = pgd_page_u(a.c, a.b, s, __builtin_amdgcn_readfirstlane(k & ~15));
-      kok[i] = page >= 0, kpos[i] = k;
-      const uint8_t *kp = a.c.k + (pgd_row(a.c, max(page, 0), g, k & ps) * HD + 8 * ko) * EB;
+      const uint8_t *kp = a.c.k + rows(b, kk + KPP * i) * (size_t)(HD * EB);
       if constexpr (EB == 1) {
-        const uint2 w = gld<uint2>(kp);
+        const uint2 w = gld<uint2>(kp + koff[i]);
         kr[i][0] = w.x, kr[i][1] = w.y;
       } else {
 #pragma unroll
         for (int e = 0; e < EB / 2; e++) {
-          const uint4 w = gld<uint4>(kp + 16 * e);
+          const uint4 w = gld<uint4>(kp + koff[i] + 16 * e);
           kr[i][4 * e] = w.x, kr[i][4 * e + 1] = w.y, kr[i][4 * e + 2] = w.z, kr[i][4 * e + 3] = w.w;
         }
       }
     }
+  };
+  auto loadv = [&](int b) {
     if (vtask) {
-      const int k = key0 + 4 * va;
-      const int page = pgd_page_u(a.c, a.b, s, __builtin_amdgcn_readfirstlane(k & ~15));
-      vok = page >= 0, vpos = k;
-      const uint8_t *vp = a.c.v + (pgd_row(a.c, max(page, 0), g, k & ps) * HD + 4 * vd) * EB;
+      const uint8_t *vp = a.c.v + rows(b, 4 * va) * (size_t)(HD * EB);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         if constexpr (EB == 1) {
-          vr[i][0] = gld<uint32_t>(vp + i * HD);
+          vr[i][0] = gld<uint32_t>(vp + voff + i * HD);
         } else if constexpr (EB == 2) {
-          const uint2 w = gld<uint2>(vp + i * HD * 2);
+          const uint2 w = gld<uint2>(vp + voff + i * HD * 2);
           vr[i][0] = w.x, vr[i][1] = w.y;
         } else {
-          const uint4 w = gld<uint4>(vp + i * HD * 4);
+          const uint4 w = gld<uint4>(vp + voff + i * HD * 4);
           vr[i][0] = w.x, vr[i][1] = w.y, vr[i][2] = w.z, vr[i][3] = w.w;
         }
       }
     }
+  };
+  /* K's scales by wave 0, V's by wave 1 */
+  auto loads = [&](int b, int w) {
     if constexpr (CT == GQ_I8_ROWS) {
-      if (tid < 2 * kKeys) {
-        const int k = key0 + tid % kKeys, page = pgd_page(a.c, a.b, s, k);
-        sc = page >= 0 && k <= pmax ? gld<float>((tid < kKeys ? a.c.ks : a.c.vs) + pgd_row(a.c, page, g, k & ps)) : 0.f;
+      if (wv == w) {
+        const int page = __shfl(pages(b), 4 * (b & 15) + (lane >> 4), 64);
+        const float d = gld<float>((w ? a.c.vs : a.c.ks) + pgd_row(a.c, max(page, 0), g, ((b * kKeys) & ps) + (lane & ps)));
+        sc = page >= 0 && b * kKeys + lane <= pmax ? d : 0.f;
       }
     }
   };
-  auto stage = [&](int buf) {
-    const uint32_t kb = (uint32_t)(buf * 2 * NK * KPL), vb = kb + NK * KPL;
+  /* the loaded K or V of block b into buffer buf; keys that do not exist are
+   * zeros */
+  auto stagek = [&](int b, int buf) {
+    const uint32_t kb = (uint32_t)(buf * 2 * NK * KPL);
+    const int ok = exists(b);
+    if (ok != 15 || b * kKeys + kKeys - 1 > pmax) {
+#pragma unroll
+      for (int i = 0; i < KI; i++) {
+        const int k = kk + KPP * i;
+        const bool there = (ok >> (k >> 4) & 1) && b * kKeys + k <= pmax;
+#pragma unroll
+        for (int e = 0; e < 2 * EB; e++) kr[i][e] = there ? kr[i][e] : 0u;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < KI; i++) {
-      const bool there = kok[i] && kpos[i] <= pmax;
-#pragma unroll
-      for (int e = 0; e < 2 * EB; e++) kr[i][e] = there ? kr[i][e] : 0u;
       const int key = kk + KPP * i;
       const uint32_t at = kb + (uint32_t)(key * HD * 2 + ((ko ^ (key & (NO - 1))) << 4));
       if constexpr (CT == GQ_BF16) {
@@ -199,11 +238,22 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         for (int n = 0; n < NK; n++) lst<gq_bf16x8>(smem, at + n * KPL, p[n]);
       }
     }
+    if constexpr (CT == GQ_I8_ROWS) {
+      if (wv == 0) lst<float>(smem, SCL + ((b & 3) * kKeys + lane) * 4, sc * a.scale);
+    }
+  };
+  auto stagev = [&](int b, int buf) {
+    const uint32_t vb = (uint32_t)((buf * 2 + 1) * NK * KPL);
+    const int ok = exists(b);
+    if (ok != 15 || b * kKeys + kKeys - 1 > pmax) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const bool there = (ok >> (va >> 2 & 3) & 1) && b * kKeys + 4 * va + i <= pmax;
+#pragma unroll
+        for (int e = 0; e < EB; e++) vr[i][e] = there ? vr[i][e] : 0u;
+      }
+    }
     if (vtask) {
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int e = 0; e < EB; e++) vr[i][e] = vok && vpos + i <= pmax ? vr[i][e] : 0u;
       const int oct = 4 * (va >> 3) + 2 * (va >> 2 & 1) + (va & 1), half = va >> 1 & 1;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
@@ -226,10 +276,9 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
           for (int n = 0; n < NK; n++) lst<uint2>(smem, at + n * KPL, p[n]);
         }
       }
-      if ((va & 3) == 0 && vd == 0) sok[buf][va >> 2] = vok;
     }
     if constexpr (CT == GQ_I8_ROWS) {
-      if (tid < 2 * kKeys) lst<float>(smem, SCL + (buf * 2 * kKeys + tid) * 4, tid < kKeys ? sc * a.scale : sc);
+      if (wv == 1) lst<float>(smem, SCL + ((4 + buf) * kKeys + lane) * 4, sc);
     }
   };
 
@@ -242,67 +291,77 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   const uint32_t kbase = (uint32_t)((32 * kh + r) * HD * 2 + ((h ^ (r & (NO - 1))) << 4));
   const uint32_t vbase = (uint32_t)(NK * KPL + r * kKeys * 2 + (((4 * kh + h) ^ ((r ^ (r >> 3)) & 7)) << 4));
 
-  auto compute = [&](int b, int buf) {
-    const int key0 = b * kKeys + 32 * kh;
-    if (key0 > whi) return; /* none of this wave's rows sees any (uniform) */
+  /* the scores of a block whose K is in buffer buf: keys 32 t + 8 (e / 4) + 4 h +
+   * e % 4 of the wave's */
+  auto scores = [&](int buf, gq_f32x16 (&st)[KT]) {
     const uint32_t at = (uint32_t)(buf * 2 * NK * KPL);
-    gq_f32x16 st[KT];
 #pragma unroll
-    for (int t = 0; t < KT; t++) {
-      st[t] = gq_f32x16{};
+    for (int t = 0; t < KT; t++) st[t] = gq_f32x16{};
 #pragma unroll
-      for (int i = 0; i < NSL; i++) {
-        gq_bf16x8 kv[NK], qv[NX];
+    for (int i = 0; i < NSL; i++) {
+      gq_bf16x8 qv[NX];
+      qv[0] = q[i][0];
+      if constexpr (NX == 3) qv[1] = q[i][1], qv[2] = lld<gq_bf16x8>(smem, qlo + RG * 1024 * i);
+#pragma unroll
+      for (int t = 0; t < KT; t++) {
+        gq_bf16x8 kv[NK];
 #pragma unroll
         for (int n = 0; n < NK; n++) kv[n] = lld<gq_bf16x8>(smem, at + (kbase ^ (32 * i)) + 32 * t * HD * 2 + n * KPL);
-        qv[0] = q[i][0];
-        if constexpr (NX == 3) qv[1] = q[i][1], qv[2] = lld<gq_bf16x8>(smem, qlo + RG * 1024 * i);
 #pragma unroll
         for (int u = 0; u < NP; u++) st[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kv[kA[W][u]], qv[kB[W][u]], st[t], 0, 0, 0);
       }
     }
-    const bool all = sok[buf][0] & sok[buf][1] & sok[buf][2] & sok[buf][3];
-    /* scores in units of log 2: key key0 + 32 t + 8 (e / 4) + 4 h + e % 4 */
-    float mb = -INFINITY;
+  };
+  /* int8: times K's scales, in units of log 2; keys that do not exist or lie past
+   * the row's position: -infinity */
+  auto mask = [&](int b, gq_f32x16 (&st)[KT]) {
+    const int key0 = b * kKeys + 32 * kh, ok = exists(b);
 #pragma unroll
     for (int t = 0; t < KT; t++) {
       if constexpr (CT == GQ_I8_ROWS) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const float4 d = lld<float4>(smem, SCL + (buf * 2 * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
+          const float4 d = lld<float4>(smem, SCL + ((b & 3) * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
           st[t][e] *= d.x, st[t][e + 1] *= d.y, st[t][e + 2] *= d.z, st[t][e + 3] *= d.w;
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) st[t][e] *= a.scale;
       }
-      if (!all || key0 + 32 * t + 31 > wlo) {
+      if (ok != 15 || key0 + 32 * t + 31 > wlo) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           const int k = 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-          st[t][e] = key0 + k <= cpos && sok[buf][(32 * kh + k) >> 4] ? st[t][e] : -INFINITY;
+          st[t][e] = key0 + k <= cpos && (ok >> ((32 * kh + k) >> 4) & 1) ? st[t][e] : -INFINITY;
         }
       }
+    }
+  };
+  gq_bf16x8 pr[2 * KT][NX];
+  float alpha;
+  bool rescale;
+  /* the probabilities of masked scores, with V's scales for int8 */
+  auto softmax = [&](int buf, gq_f32x16 (&st)[KT]) {
+    float mb = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT; t++)
 #pragma unroll
       for (int e = 0; e < 16; e++) mb = fmaxf(mb, st[t][e]);
-    }
-    mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+    mb = max_halves(mb);
+    if constexpr (CT != GQ_I8_ROWS) mb *= a.scale;
     const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - ms);
+    alpha = __builtin_amdgcn_exp2f(m - ms);
+    rescale = __ballot(mn > m) != 0; /* some row's maximum has risen (alpha is 1 in the others) */
     m = mn;
     l *= alpha;
-    gq_bf16x8 ps[2 * KT][NX];
 #pragma unroll
     for (int t = 0; t < KT; t++) {
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        st[t][e] = __builtin_amdgcn_exp2f(st[t][e] - ms);
+        st[t][e] = __builtin_amdgcn_exp2f(CT == GQ_I8_ROWS ? st[t][e] - ms : __builtin_fmaf(st[t][e], a.scale, -ms));
         l += st[t][e];
       }
       if constexpr (CT == GQ_I8_ROWS) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const float4 d = lld<float4>(smem, SCL + (buf * 2 * kKeys + kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
+          const float4 d = lld<float4>(smem, SCL + ((4 + buf) * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
           st[t][e] *= d.x, st[t][e + 1] *= d.y, st[t][e + 2] *= d.z, st[t][e + 3] *= d.w;
         }
       }
@@ -311,12 +370,24 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = st[t][8 * u + e];
-        split8<NX>(x, ps[2 * t + u]);
+        split8<NX>(x, pr[2 * t + u]);
       }
+    }
+  };
+  auto output = [&](int buf) {
+    const uint32_t at = (uint32_t)(buf * 2 * NK * KPL);
+    /* fp32 results: the block's P V in accumulators of its own, so that O takes
+     * one rounding a block and not one a product */
+    constexpr bool OWN = NX == 3;
+    if (!OWN && rescale) {
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[d][e] *= alpha;
     }
 #pragma unroll
     for (int d = 0; d < ND; d++) {
-      gq_f32x16 pv = gq_f32x16{};
+      gq_f32x16 pv = OWN ? gq_f32x16{} : o[d];
 #pragma unroll
       for (int t = 0; t < 2 * KT; t++) {
         gq_bf16x8 vv[NK];
@@ -324,36 +395,158 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         for (int n = 0; n < NK; n++)
           vv[n] = lld<gq_bf16x8>(smem, at + (vbase ^ (((4 * d & 7) ^ (2 * t)) << 4)) + n * KPL + 32 * d * kKeys * 2);
 #pragma unroll
-        for (int u = 0; u < NP; u++) pv = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv[kA[W][u]], ps[t][kB[W][u]], pv, 0, 0, 0);
+        for (int u = 0; u < NP; u++) pv = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv[kA[W][u]], pr[t][kB[W][u]], pv, 0, 0, 0);
       }
+      if constexpr (OWN) {
 #pragma unroll
-      for (int e = 0; e < 16; e++) o[d][e] = __builtin_fmaf(o[d][e], alpha, pv[e]);
+        for (int e = 0; e < 16; e++) o[d][e] = __builtin_fmaf(o[d][e], alpha, pv[e]);
+      } else {
+        o[d] = pv;
+      }
     }
   };
 
-  /* past the end the last block loads again: under a condition the loads would
-   * leave registers undefined (decode_kernel) */
-  if (nblk > 0) {
-    load(0);
-    if constexpr (NB == 2) {
-      stage(0);
-      load(min(1, nblk - 1));
+  /* Loads past the end take the last block again: under a condition they would
+   * leave registers undefined (decode_kernel). */
+  const int bl = nblk - 1;
+  auto turn = [&](int b) { /* pages for the blocks from b on */
+    if ((b & 15) == 0) pg0 = pg1, pgn = b >> 4, pg1 = lookup(pgn + 1);
+  };
+  if (nblk > 0) pg0 = lookup(0), pg1 = lookup(1);
+  if constexpr (PIPE) {
+    /* Block b + 1's scores and b's softmax together: a wave's matrix instructions
+     * run under its own vector ones.  K is a block further ahead than V. */
+    if (nblk > 0) {
+      gq_f32x16 sa[KT], sb[KT];
+      loadk(0), loads(0, 0), loadv(0), loads(0, 1);
+      stagek(0, 0), stagev(0, 0);
+      loadk(min(1, bl)), loads(min(1, bl), 0), loadv(min(1, bl)), loads(min(1, bl), 1);
+      stagek(min(1, bl), 1);
+      loadk(min(2, bl)), loads(min(2, bl), 0);
       __syncthreads();
-      for (int b = 0; b < nblk; b++) {
-        stage((b + 1) & 1); /* last read before the barrier below */
-        load(min(b + 2, nblk - 1));
-        compute(b, b & 1);
+      scores(0, sa);
+      __syncthreads(); /* K of block 0 has been read */
+      /* before it K of b and b + 1 and V of b are in LDS, K of b + 2 and V of b + 1
+       * in registers.  Written in the order in which it is to run: four LDS
+       * operands ahead of the matrix instructions, a piece of the softmax after
+       * each (the compiler's own order waits for every operand). */
+      auto body = [&](int b, gq_f32x16 (&cur)[KT], gq_f32x16 (&next)[KT]) {
+        constexpr int N = KT * NSL, J = 4 * KT, N2 = 2 * KT * ND, A = 4; /* A operands ahead */
+        mask(b, cur);
+        const uint32_t kat = (uint32_t)(((b + 1) & 1) * 2 * KPL) + kbase, vat = (uint32_t)((b & 1) * 2 * KPL) + vbase;
+        const uint32_t sat = (uint32_t)(SCL + (4 + (b & 1)) * kKeys * 4 + (32 * kh + 4 * h) * 4);
+        auto kop = [&](int i) { return lld<gq_bf16x8>(smem, (kat ^ (32 * (i / KT))) + 32 * (i % KT) * HD * 2); };
+        auto vop = [&](int i) {
+          return lld<gq_bf16x8>(smem, (vat ^ (((4 * (i % ND) & 7) ^ (2 * (i / ND))) << 4)) + 32 * (i % ND) * kKeys * 2);
+        };
+        gq_bf16x8 w[A];
+#pragma unroll
+        for (int i = 0; i < A; i++) w[i] = kop(i);
+        float ms = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          __builtin_amdgcn_sched_barrier(0);
+          next[i % KT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[i % A], q[i / KT][0], i < KT ? gq_f32x16{} : next[i % KT], 0, 0, 0);
+          if (i + A < N) w[i % A] = kop(i + A);
+          if (i == 0) {
+            float mb = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+              for (int e = 0; e < 16; e++) mb = fmaxf(mb, cur[t][e]);
+            mb = max_halves(mb);
+            if constexpr (CT != GQ_I8_ROWS) mb *= a.scale;
+            const float mn = fmaxf(m, mb);
+            ms = mn == -INFINITY ? 0.f : mn;
+            alpha = __builtin_amdgcn_exp2f(m - ms);
+            rescale = __ballot(mn > m) != 0;
+            m = mn, l *= alpha;
+          }
+#pragma unroll
+          for (int c = (i - 1) * J / (N - 1); i && c < i * J / (N - 1); c++) { /* scores 4 c .. + 3 */
+            const int t = c / 4, e0 = 4 * (c % 4);
+#pragma unroll
+            for (int e = e0; e < e0 + 4; e++) {
+              cur[t][e] = __builtin_amdgcn_exp2f(CT == GQ_I8_ROWS ? cur[t][e] - ms : __builtin_fmaf(cur[t][e], a.scale, -ms));
+              l += cur[t][e];
+            }
+            if constexpr (CT == GQ_I8_ROWS) {
+              const float4 d = lld<float4>(smem, sat + (32 * t + 2 * e0) * 4);
+              cur[t][e0] *= d.x, cur[t][e0 + 1] *= d.y, cur[t][e0 + 2] *= d.z, cur[t][e0 + 3] *= d.w;
+            }
+            if (c & 1) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; e++) x[e] = cur[t][e0 - 4 + e];
+              split8<1>(x, pr[c / 2]);
+              pin(pr[c / 2][0], l); /* here and not where they are used */
+            }
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        stagek(min(b + 2, bl), b & 1), stagev(min(b + 1, bl), (b + 1) & 1);
+        loadk(min(b + 3, bl)), loads(min(b + 3, bl), 0);
+        loadv(min(b + 2, bl)), loads(min(b + 2, bl), 1);
+        if (rescale) {
+#pragma unroll
+          for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < A; i++) w[i] = vop(i);
+#pragma unroll
+        for (int i = 0; i < N2; i++) {
+          __builtin_amdgcn_sched_barrier(0);
+          o[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[i % A], pr[i / ND][0], o[i % ND], 0, 0, 0);
+          if (i + A < N2) w[i % A] = vop(i + A);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        turn(b + 1);
+        __syncthreads();
+      };
+      for (int b = 0;;) {
+        body(b, sa, sb);
+        if (++b >= nblk) break;
+        body(b, sb, sa);
+        if (++b >= nblk) break;
+      }
+    }
+  } else {
+    auto compute = [&](int b, int buf) {
+      if (b * kKeys + 32 * kh > whi) return; /* none of this wave's rows sees any (uniform) */
+      gq_f32x16 st[KT];
+      scores(buf, st);
+      mask(b, st);
+      softmax(buf, st);
+      output(buf);
+    };
+    auto load = [&](int b) { loadk(b), loads(b, 0), loadv(b), loads(b, 1); };
+    if (nblk > 0) {
+      load(0);
+      if constexpr (NB == 2) {
+        stagek(0, 0), stagev(0, 0);
+        load(min(1, bl));
+        __syncthreads();
+        for (int b = 0; b < nblk; b++) {
+          const int n = min(b + 1, bl);
+          stagek(n, (b + 1) & 1), stagev(n, (b + 1) & 1); /* last read before the barrier below */
+          load(min(b + 2, bl));
+          compute(b, b & 1);
+          turn(b + 1);
+          __syncthreads();
+        }
+      } else {
+        for (int b = 0; b < nblk; b++) {
+          __syncthreads(); /* the planes are free */
+          stagek(b, 0), stagev(b, 0);
+          __syncthreads();
+          load(min(b + 1, bl));
+          compute(b, 0);
+          turn(b + 1);
+        }
         __syncthreads();
       }
-    } else {
-      for (int b = 0; b < nblk; b++) {
-        __syncthreads(); /* the planes are free */
-        stage(0);
-        __syncthreads();
-        load(min(b + 1, nblk - 1));
-        compute(b, 0);
-      }
-      __syncthreads();
     }
   }
   l += __shfl_xor(l, 32, 64);
