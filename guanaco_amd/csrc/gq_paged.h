@@ -134,11 +134,18 @@ struct AttArgs {
   void *out;
   float *part_o, *part_ml; /* [row][head][nch][hd] and [..][2] */
   int n_heads, G, qs, os;
-  int nch, chunk; /* decode: parts of at most `chunk` keys, a multiple of 128 */
+  int nch, chunk; /* at most nch parts, of at most `chunk` keys (decode: a multiple of 128) or blocks of 64 keys */
   float scale;    /* log2(e) / sqrt(head_dim) */
 };
 
-/* gq_paged_prompt.hip: every new token's attention; 0, or -4 */
-int gq_launch_paged_prompt(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu, hipStream_t s);
+/* gq_paged_prompt.hip: every new token's attention.  The shape of its launch:
+ * rows of a tile, blocks of 64 keys a part, at most so many parts (more than
+ * one: part_o and part_ml hold n_tokens rows), workgroups (0: too many). */
+struct PromptShape {
+  int rows, span, parts;
+  unsigned blocks;
+};
+PromptShape gq_paged_prompt_shape(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu);
+int gq_launch_paged_prompt(const AttArgs &a, int cache, int xtype, int head_dim, const PromptShape &f, hipStream_t s);
 
 #endif

@@ -750,5 +750,14 @@ extern "C" int gq_hip_paged_prompt_dev(gq_ctx *c, const gq_pages *p, const gq_ba
   if (int rc = att_args(c, p, b, xtype, n_heads, q, q_stride, out, out_stride, a)) return rc > 0 ? 0 : rc;
   const GqCtxInfo ci = gq_ctx_info(c);
   GqDeviceGuard guard(ci.dev);
-  return gq_launch_paged_prompt(a, p->dtype, xtype, p->head_dim, ci.n_cu, ci.stream) ? gq_ctx_fail(c, -4, "paged prompt launch") : 0;
+  const PromptShape f = gq_paged_prompt_shape(a, p->dtype, xtype, p->head_dim, ci.n_cu);
+  if (!f.blocks) return gq_ctx_fail(c, -1, "paged prompt: the batch passes a launch");
+  a.nch = f.parts, a.chunk = f.span;
+  if (a.nch > 1) {
+    const size_t rows = (size_t)b->n_tokens * n_heads * a.nch;
+    a.part_o = (float *)gq_ctx_paged_ws(c, sizeof(float) * rows * (p->head_dim + 2));
+    if (!a.part_o) return -4;
+    a.part_ml = a.part_o + rows * p->head_dim;
+  }
+  return gq_launch_paged_prompt(a, p->dtype, xtype, p->head_dim, f, ci.stream) ? gq_ctx_fail(c, -4, "paged prompt launch") : 0;
 }

@@ -13,17 +13,37 @@ typedef float gq_f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kPThreads = 512, kKeys = 64;
 
-/* The sequence and tile of a workgroup: tiles of tpt tokens, sequence after
- * sequence; s = n_seqs past the last one. */
-__device__ __forceinline__ void find_tile(const PgdBatch &b, int tpt, int id, int &s, int &tile) {
+/* A tile of query rows: up to tpt new tokens of a sequence, from its t0-th on,
+ * packed from row `row` on; p0 positions are before the sequence's first. */
+struct Tile {
+  int s, row, t0, n, p0; /* n 0: there is none */
+};
+/* The id-th tile: of 64 sequences at a time the longest first, and of each its
+ * last one first, so that what runs longest starts first (uniform in the wave). */
+__device__ __forceinline__ Tile find_tile(const PgdBatch &b, int tpt, int id) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int s0 = 0; s0 < b.n_seqs; s0 += GQ_WAVE) {
-    const int q = s0 + lane, qc = min(q, b.n_seqs - 1);
+    const int q = s0 + lane, qc = min(q, b.n_seqs - 1), cnt = min(GQ_WAVE, b.n_seqs - s0);
     int r0 = qc, r1 = qc + 1;
     if (b.first) r0 = gld<int>(b.first + qc), r1 = gld<int>(b.first + qc + 1);
+    int p0 = gld<int>(b.pos + qc);
     const bool in = q < b.n_seqs && r0 >= 0 && r1 <= b.n_tokens && r1 > r0;
-    int c = in ? (r1 - r0 + tpt - 1) / tpt : 0;
+    if (!in) r0 = r1 = 0;
+    int sq = q;
+    if (cnt > 1) { /* lane i: the i-th longest */
+      const int len = in ? max(p0, 0) + (r1 - r0) : -1;
+      int rank = 0;
+      for (int i = 0; i < cnt; i++) {
+        const int u = __builtin_amdgcn_readlane(len, i);
+        rank += u > len || (u == len && i < lane);
+      }
+      const int to = 4 * (lane < cnt ? rank : lane);
+      sq = __builtin_amdgcn_ds_permute(to, sq), p0 = __builtin_amdgcn_ds_permute(to, p0);
+      r0 = __builtin_amdgcn_ds_permute(to, r0), r1 = __builtin_amdgcn_ds_permute(to, r1);
+    }
+    const int own = (r1 - r0 + tpt - 1) / tpt;
+    int c = own;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int u = __shfl_up(c, o, 64);
@@ -32,20 +52,33 @@ __device__ __forceinline__ void find_tile(const PgdBatch &b, int tpt, int id, in
     const uint64_t hit = __ballot(before + c > id);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      s = s0 + l;
-      tile = id - before - (l ? __shfl(c, l - 1, 64) : 0);
-      return;
+      const int t0 = (before + __builtin_amdgcn_readlane(c, l) - 1 - id) * tpt;
+      r0 = __builtin_amdgcn_readlane(r0, l), r1 = __builtin_amdgcn_readlane(r1, l);
+      return Tile{__builtin_amdgcn_readlane(sq, l), r0 + t0, t0, min(tpt, r1 - r0 - t0), __builtin_amdgcn_readlane(p0, l)};
     }
-    before += __shfl(c, 63, 64);
+    before += __builtin_amdgcn_readlane(c, 63);
   }
-  s = b.n_seqs, tile = 0;
+  return Tile{0, 0, 0, 0, 0};
 }
 
+/* Blocks of 64 keys that a tile sees, and the parts that they come in: of at
+ * most a.chunk, evenly. */
+__device__ __forceinline__ int2 tile_blocks(const AttArgs &a, int p0, int last) {
+  const int pmax = p0 < 0 ? -1 : min(p0 + last, a.b.max_len - 1), n = max(0, (pmax + kKeys) / kKeys);
+  return make_int2(n, max(1, (n + a.chunk - 1) / a.chunk));
+}
+
+/* lanes 32 .. 63 of a against lanes 0 .. 31 of b */
+__device__ __forceinline__ void swap_halves(float &a, float &b) {
+  const auto w = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+  const uint32_t x = w[0], y = w[1]; /* a bit cast of w[1] itself would read w[0] */
+  a = __builtin_bit_cast(float, x), b = __builtin_bit_cast(float, y);
+}
 /* the larger of a lane's value and that of the lane 32 away */
 __device__ __forceinline__ float max_halves(float v) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
-  const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return fmaxf(__builtin_bit_cast(float, w[0]), __builtin_bit_cast(float, w[1]));
+  float w = v;
+  swap_halves(v, w);
+  return fmaxf(v, w);
 }
 
 __device__ __forceinline__ void pin(gq_bf16x8 &v, float &f) {
@@ -69,15 +102,20 @@ __device__ __forceinline__ void pin(gq_bf16x8 &v, float &f) {
  *                  way); lane (r, h) holds row r's outputs, so the softmax's
  *                  rescale and the division stay in the lane.
  * The blocks are loaded a block ahead into registers, turned into bf16 and put
- * into LDS, octets (16 bytes) XOR-swizzled by the row.  bf16 values and int8
- * codes are exact there (the scales multiply scores and probabilities); fp32
- * accuracy is kept by splitting an fp32 operand x into three bf16 numbers that
- * sum to it, and keeping the partial products that are not below 2^-24: three
- * for fp32 queries over a bf16 or int8 cache, six over an fp32 one.  bf16
- * queries take bf16 probabilities, and round an fp32 cache's values to bf16.
+ * into LDS, octets (16 bytes) XOR-swizzled by the row.  fp32 queries keep fp32
+ * accuracy: bf16 values and int8 codes are exact there (the scales multiply
+ * scores and probabilities), and an fp32 operand is split into three bf16
+ * numbers that sum to it, of whose products those not below 2^-24 are kept:
+ * three over a bf16 or int8 cache, six over an fp32 one.  bf16 queries, whose
+ * results are bf16, take probabilities rounded to bf16 and an fp32 or int8
+ * cache's values likewise: as exact as the queries themselves, for one product,
+ * and for int8 without 64 products by scales a lane and block (2.5 -> 1.8 us).
  *
- * Keys that do not exist are zeros in LDS and masked, so that what stale
- * memory holds cannot reach a sum. */
+ * Keys that do not exist are masked, and their V zeros in LDS, so that what stale
+ * memory holds cannot reach a sum.
+ *
+ * The blocks of a tile come in parts of at most a.chunk, a workgroup each, where
+ * the tiles alone would leave CUs idle; prompt_merge_kernel joins them. */
 template <int CT, int XT, int HD, int RG, int KH>
 __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_kernel(AttArgs a) {
   static_assert(RG * KH * GQ_WAVE == kPThreads, "eight waves");
@@ -88,6 +126,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   constexpr int W = NP == 6 ? 2 : NP == 3 ? 1 : 0;
   constexpr int NB = NK == 1 ? 2 : 1;        /* blocks in LDS */
   constexpr bool PIPE = NX == 1;
+  constexpr bool CODES = CT == GQ_I8_ROWS && NX == 3; /* int8 codes in LDS, scales apart; else values */
+  constexpr bool VALUES = CT == GQ_I8_ROWS && NX == 1;
   constexpr int EB = pgd_bytes(CT);
   constexpr int NO = HD / 8;                 /* octets of a K row */
   constexpr int NSL = HD / 16, ND = HD / 32; /* dim slices of S^T, dim tiles of O^T */
@@ -95,54 +135,61 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   constexpr int KPL = kKeys * HD * 2;        /* bytes of one plane */
   constexpr int KI = kKeys * NO / kPThreads; /* K octets a thread */
   constexpr int KPP = kPThreads / NO;        /* keys a pass of them */
+  constexpr int KW = 2 * EB + VALUES, VW = EB + VALUES;
   constexpr int VTH = 16 * HD / 4;           /* threads with four keys x four dims of V */
   constexpr int NQ = NX == 3 ? 2 : 1;        /* planes of Q in registers; the third in LDS */
   constexpr int QLO = NB * 2 * NK * KPL, SCL = QLO + (NX == 3 ? RG * NSL * 1024 : 0);
-  constexpr int LDS = SCL + (CT == GQ_I8_ROWS ? (4 + NB) * kKeys * 4 : 0); /* scales: four blocks of K's, NB of V's */
-  static_assert(KH == 1 || LDS >= RG * 64 * 4 * (ND * 16 + 2), "the halves' exchange fits");
+  constexpr int LDS = std::max(SCL + (CODES ? (4 + NB) * kKeys * 4 : 0), /* scales: four blocks of K's, NB of V's */
+                               KH == 2 ? RG * 64 * 4 * (ND * 16 + 2) : 0);          /* the halves' exchange */
   __shared__ __attribute__((aligned(16))) uint8_t smem_[LDS];
   GQ_LDS uint8_t *smem = (GQ_LDS uint8_t *)smem_;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wv / KH, kh = wv % KH;
   const int G = a.G, tpt = 32 * RG / G;
-  const int g = blockIdx.x % a.c.n_kv;
-  int s, tile;
-  find_tile(a.b, tpt, (int)(gridDim.x / a.c.n_kv - 1 - blockIdx.x / a.c.n_kv), s, tile);
-  s = __builtin_amdgcn_readfirstlane(s), tile = __builtin_amdgcn_readfirstlane(tile);
-  if (s >= a.b.n_seqs) return;
-  const int2 rn = pgd_rows(a.b, s);
-  const int p0 = gq_sld<int>(a.b.pos + s), t0 = tile * tpt, nt = min(tpt, rn.y - t0);
+  int bid = blockIdx.x;
+  const int g = bid % a.c.n_kv;
+  bid /= a.c.n_kv;
+  const int part = bid % a.nch;
+  const Tile tl = find_tile(a.b, tpt, bid / a.nch);
+  if (!tl.n) return;
+  const int s = tl.s;
   /* position that a row of the tile sees last; none of an idle sequence */
-  auto sees = [&](int row) { return p0 < 0 ? -1 : min(p0 + t0 + min(row / G, nt - 1), a.b.max_len - 1); };
-  const int pmax = sees(32 * RG - 1), nblk = (pmax + kKeys) / kKeys; /* 0 for -1 */
-  const int row = 32 * rg + r, tok = min(row / G, nt - 1), qh = g * G + row % G;
-  const bool live = row < tpt * G && row / G < nt;
+  auto sees = [&](int row) { return tl.p0 < 0 ? -1 : min(tl.p0 + tl.t0 + min(row / G, tl.n - 1), a.b.max_len - 1); };
+  const int2 bp = tile_blocks(a, tl.p0, tl.t0 + tl.n - 1);
+  if (part >= bp.y) return;
+  const int b0 = (int)((long long)bp.x * part / bp.y), b1 = (int)((long long)bp.x * (part + 1) / bp.y); /* this part's blocks */
+  const int pmax = sees(32 * RG - 1);
+  const int row = 32 * rg + r, tok = min(row / G, tl.n - 1), qh = g * G + row % G;
+  const bool live = row < tpt * G && row / G < tl.n;
   const int cpos = sees(row), wlo = sees(32 * rg), whi = sees(32 * rg + 31);
 
   /* this row's query: dims 16 i + 8 h .. + 7 */
   gq_bf16x8 q[NSL][NQ];
   const uint32_t qlo = (uint32_t)(QLO + (rg * 64 + lane) * 16);
+  auto query = [&] {
+    const size_t at = (size_t)(tl.row + tok) * a.qs + (size_t)qh * HD + 8 * h;
 #pragma unroll
-  for (int i = 0; i < NSL; i++) {
-    float x[8];
-    pgd_load8<XT>(a.q, (size_t)(rn.x + t0 + tok) * a.qs + (size_t)qh * HD + 16 * i + 8 * h, x);
-    if constexpr (NX == 3) {
-      gq_bf16x8 p[3];
-      split8<3>(x, p);
-      q[i][0] = p[0], q[i][1] = p[1];
-      if (kh == 0) lst<gq_bf16x8>(smem, qlo + RG * 1024 * i, p[2]);
-    } else {
-      split8<1>(x, q[i]);
+    for (int i = 0; i < NSL; i++) {
+      if constexpr (NX == 3) {
+        float x[8];
+        pgd_load8<XT>(a.q, at + 16 * i, x);
+        gq_bf16x8 p[3];
+        split8<3>(x, p);
+        q[i][0] = p[0], q[i][1] = p[1];
+        if (kh == 0) lst<gq_bf16x8>(smem, qlo + RG * 1024 * i, p[2]);
+      } else {
+        q[i][0] = gld<gq_bf16x8>((const uint16_t *)a.q + at + 16 * i);
+      }
     }
-  }
+  };
 
   /* staging: K octet ko of keys kk, kk + KPP ..; V dims 4 vd .. + 3 of keys 4
    * va .. + 3; a wave's keys are of one 16-key group each time, and so of one
    * page. */
   const int ko = tid % NO, kk = tid / NO, vd = tid % (HD / 4), va = tid / (HD / 4);
   const bool vtask = VTH == kPThreads || tid < VTH;
-  uint32_t kr[KI][2 * EB], vr[4][EB]; /* raw dwords */
-  float sc = 0.f;                     /* tid < 128: the scale of key tid % 64, K's then V's */
+  uint32_t kr[KI][KW], vr[4][VW]; /* raw dwords, and the scales of VALUES */
+  float sc = 0.f;                     /* int8: the scale of key `lane`, K's in wave 0 and V's in wave 1 */
   const int ps = (1 << a.c.lg) - 1;
   uint32_t koff[KI]; /* within a page's rows for the head, from the block's first slot */
 #pragma unroll
@@ -163,10 +210,12 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     const int page = __builtin_amdgcn_readlane(pages(b), __builtin_amdgcn_readfirstlane(4 * (b & 15) + (key >> 4)));
     return pgd_row(a.c, max(page, 0), g, (b * kKeys) & ps);
   };
-  auto loadk = [&](int b) {
+  auto loadk = [&](int b, uint32_t (&kr)[KI][KW]) {
 #pragma unroll
     for (int i = 0; i < KI; i++) {
-      const uint8_t *kp = a.c.k + rows(b, kk + KPP * i) * (size_t)(HD * EB);
+      const size_t at = rows(b, kk + KPP * i);
+      const uint8_t *kp = a.c.k + at * (size_t)(HD * EB);
+      if constexpr (VALUES) kr[i][2] = gld<uint32_t>(a.c.ks + at + ((kk + KPP * i) & ps));
       if constexpr (EB == 1) {
         const uint2 w = gld<uint2>(kp + koff[i]);
         kr[i][0] = w.x, kr[i][1] = w.y;
@@ -179,9 +228,14 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       }
     }
   };
-  auto loadv = [&](int b) {
+  auto loadv = [&](int b, uint32_t (&vr)[4][VW]) {
     if (vtask) {
-      const uint8_t *vp = a.c.v + rows(b, 4 * va) * (size_t)(HD * EB);
+      const size_t at = rows(b, 4 * va);
+      const uint8_t *vp = a.c.v + at * (size_t)(HD * EB);
+      if constexpr (VALUES) {
+        const uint4 d = gld<uint4>(a.c.vs + at + ((4 * va) & ps));
+        vr[0][1] = d.x, vr[1][1] = d.y, vr[2][1] = d.z, vr[3][1] = d.w;
+      }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         if constexpr (EB == 1) {
@@ -196,9 +250,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       }
     }
   };
-  /* K's scales by wave 0, V's by wave 1 */
-  auto loads = [&](int b, int w) {
-    if constexpr (CT == GQ_I8_ROWS) {
+  auto loads = [&](int b, int w, float &sc) {
+    if constexpr (CODES) {
       if (wv == w) {
         const int page = __shfl(pages(b), 4 * (b & 15) + (lane >> 4), 64);
         const float d = gld<float>((w ? a.c.vs : a.c.ks) + pgd_row(a.c, max(page, 0), g, ((b * kKeys) & ps) + (lane & ps)));
@@ -206,28 +259,26 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       }
     }
   };
-  /* the loaded K or V of block b into buffer buf; keys that do not exist are
-   * zeros */
-  auto stagek = [&](int b, int buf) {
+  /* the loaded K or V of block b into buffer buf; V's rows that do not exist are
+   * zeros (K's scores are masked) */
+  auto stagek = [&](int b, int buf, uint32_t (&kr)[KI][KW], float sc) {
     const uint32_t kb = (uint32_t)(buf * 2 * NK * KPL);
-    const int ok = exists(b);
-    if (ok != 15 || b * kKeys + kKeys - 1 > pmax) {
-#pragma unroll
-      for (int i = 0; i < KI; i++) {
-        const int k = kk + KPP * i;
-        const bool there = (ok >> (k >> 4) & 1) && b * kKeys + k <= pmax;
-#pragma unroll
-        for (int e = 0; e < 2 * EB; e++) kr[i][e] = there ? kr[i][e] : 0u;
-      }
-    }
 #pragma unroll
     for (int i = 0; i < KI; i++) {
       const int key = kk + KPP * i;
       const uint32_t at = kb + (uint32_t)(key * HD * 2 + ((ko ^ (key & (NO - 1))) << 4));
       if constexpr (CT == GQ_BF16) {
         lst<uint4>(smem, at, make_uint4(kr[i][0], kr[i][1], kr[i][2], kr[i][3]));
-      } else if constexpr (CT == GQ_I8_ROWS) {
+      } else if constexpr (CODES) {
         lst<gq_bf16x8>(smem, at, codes8(kr[i][0], kr[i][1]));
+      } else if constexpr (VALUES) {
+        const float d = __builtin_bit_cast(float, kr[i][2]);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = i8f(kr[i][e >> 2], e & 3) * d;
+        gq_bf16x8 p[1];
+        split8<1>(x, p);
+        lst<gq_bf16x8>(smem, at, p[0]);
       } else {
         float x[8];
 #pragma unroll
@@ -238,11 +289,11 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         for (int n = 0; n < NK; n++) lst<gq_bf16x8>(smem, at + n * KPL, p[n]);
       }
     }
-    if constexpr (CT == GQ_I8_ROWS) {
+    if constexpr (CODES) {
       if (wv == 0) lst<float>(smem, SCL + ((b & 3) * kKeys + lane) * 4, sc * a.scale);
     }
   };
-  auto stagev = [&](int b, int buf) {
+  auto stagev = [&](int b, int buf, uint32_t (&vr)[4][VW], float sc) {
     const uint32_t vb = (uint32_t)((buf * 2 + 1) * NK * KPL);
     const int ok = exists(b);
     if (ok != 15 || b * kKeys + kKeys - 1 > pmax) {
@@ -250,7 +301,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       for (int i = 0; i < 4; i++) {
         const bool there = (ok >> (va >> 2 & 3) & 1) && b * kKeys + 4 * va + i <= pmax;
 #pragma unroll
-        for (int e = 0; e < EB; e++) vr[i][e] = there ? vr[i][e] : 0u;
+        for (int e = 0; e < VW; e++) vr[i][e] = there ? vr[i][e] : 0u;
       }
     }
     if (vtask) {
@@ -264,7 +315,13 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
           lst<uint2>(smem, at, make_uint2(__builtin_amdgcn_perm(vr[1][j / 2], vr[0][j / 2], sel),
                                           __builtin_amdgcn_perm(vr[3][j / 2], vr[2][j / 2], sel)));
         } else if constexpr (CT == GQ_I8_ROWS) {
-          lst<uint2>(smem, at, make_uint2(pgd_pack(i8f(vr[0][0], j), i8f(vr[1][0], j)), pgd_pack(i8f(vr[2][0], j), i8f(vr[3][0], j))));
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            x[i] = i8f(vr[i][0], j);
+            if constexpr (VALUES) x[i] *= __builtin_bit_cast(float, vr[i][1]);
+          }
+          lst<uint2>(smem, at, make_uint2(pgd_pack(x[0], x[1]), pgd_pack(x[2], x[3])));
         } else {
           float x[4];
 #pragma unroll
@@ -277,7 +334,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         }
       }
     }
-    if constexpr (CT == GQ_I8_ROWS) {
+    if constexpr (CODES) {
       if (wv == 1) lst<float>(smem, SCL + ((4 + buf) * kKeys + lane) * 4, sc);
     }
   };
@@ -318,7 +375,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     const int key0 = b * kKeys + 32 * kh, ok = exists(b);
 #pragma unroll
     for (int t = 0; t < KT; t++) {
-      if constexpr (CT == GQ_I8_ROWS) {
+      if constexpr (CODES) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 d = lld<float4>(smem, SCL + ((b & 3) * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
@@ -345,7 +402,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
       for (int e = 0; e < 16; e++) mb = fmaxf(mb, st[t][e]);
     mb = max_halves(mb);
-    if constexpr (CT != GQ_I8_ROWS) mb *= a.scale;
+    if constexpr (!CODES) mb *= a.scale;
     const float mn = fmaxf(m, mb), ms = mn == -INFINITY ? 0.f : mn;
     alpha = __builtin_amdgcn_exp2f(m - ms);
     rescale = __ballot(mn > m) != 0; /* some row's maximum has risen (alpha is 1 in the others) */
@@ -355,10 +412,10 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     for (int t = 0; t < KT; t++) {
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        st[t][e] = __builtin_amdgcn_exp2f(CT == GQ_I8_ROWS ? st[t][e] - ms : __builtin_fmaf(st[t][e], a.scale, -ms));
+        st[t][e] = __builtin_amdgcn_exp2f(CODES ? st[t][e] - ms : __builtin_fmaf(st[t][e], a.scale, -ms));
         l += st[t][e];
       }
-      if constexpr (CT == GQ_I8_ROWS) {
+      if constexpr (CODES) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 d = lld<float4>(smem, SCL + ((4 + buf) * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
@@ -408,23 +465,29 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 
   /* Loads past the end take the last block again: under a condition they would
    * leave registers undefined (decode_kernel). */
-  const int bl = nblk - 1;
+  const int bl = b1 - 1;
   auto turn = [&](int b) { /* pages for the blocks from b on */
     if ((b & 15) == 0) pg0 = pg1, pgn = b >> 4, pg1 = lookup(pgn + 1);
   };
-  if (nblk > 0) pg0 = lookup(0), pg1 = lookup(1);
+  if (b0 < b1) pgn = b0 >> 4, pg0 = lookup(pgn), pg1 = lookup(pgn + 1);
   if constexpr (PIPE) {
     /* Block b + 1's scores and b's softmax together: a wave's matrix instructions
      * run under its own vector ones.  K is a block further ahead than V. */
-    if (nblk > 0) {
+    if (b0 < b1) {
       gq_f32x16 sa[KT], sb[KT];
-      loadk(0), loads(0, 0), loadv(0), loads(0, 1);
-      stagek(0, 0), stagev(0, 0);
-      loadk(min(1, bl)), loads(min(1, bl), 0), loadv(min(1, bl)), loads(min(1, bl), 1);
-      stagek(min(1, bl), 1);
-      loadk(min(2, bl)), loads(min(2, bl), 0);
+      {
+        uint32_t k0[KI][KW], k1[KI][KW], v0[4][VW];
+        float c0 = 0.f, c1 = 0.f;
+        const int n1 = min(b0 + 1, bl), n2 = min(b0 + 2, bl);
+        loadk(b0, k0), loads(b0, 0, c0), loadv(b0, v0), loads(b0, 1, c0);
+        loadk(n1, k1), loads(n1, 0, c1), loadv(n1, vr), loads(n1, 1, sc);
+        loadk(n2, kr), loads(n2, 0, sc);
+        query();
+        stagek(b0, b0 & 1, k0, c0), stagev(b0, b0 & 1, v0, c0);
+        stagek(n1, (b0 + 1) & 1, k1, c1);
+      }
       __syncthreads();
-      scores(0, sa);
+      scores(b0 & 1, sa);
       __syncthreads(); /* K of block 0 has been read */
       /* before it K of b and b + 1 and V of b are in LDS, K of b + 2 and V of b + 1
        * in registers.  Written in the order in which it is to run: four LDS
@@ -434,7 +497,6 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         constexpr int N = KT * NSL, J = 4 * KT, N2 = 2 * KT * ND, A = 4; /* A operands ahead */
         mask(b, cur);
         const uint32_t kat = (uint32_t)(((b + 1) & 1) * 2 * KPL) + kbase, vat = (uint32_t)((b & 1) * 2 * KPL) + vbase;
-        const uint32_t sat = (uint32_t)(SCL + (4 + (b & 1)) * kKeys * 4 + (32 * kh + 4 * h) * 4);
         auto kop = [&](int i) { return lld<gq_bf16x8>(smem, (kat ^ (32 * (i / KT))) + 32 * (i % KT) * HD * 2); };
         auto vop = [&](int i) {
           return lld<gq_bf16x8>(smem, (vat ^ (((4 * (i % ND) & 7) ^ (2 * (i / ND))) << 4)) + 32 * (i % ND) * kKeys * 2);
@@ -455,7 +517,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
               for (int e = 0; e < 16; e++) mb = fmaxf(mb, cur[t][e]);
             mb = max_halves(mb);
-            if constexpr (CT != GQ_I8_ROWS) mb *= a.scale;
+            mb *= a.scale;
             const float mn = fmaxf(m, mb);
             ms = mn == -INFINITY ? 0.f : mn;
             alpha = __builtin_amdgcn_exp2f(m - ms);
@@ -467,12 +529,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
             const int t = c / 4, e0 = 4 * (c % 4);
 #pragma unroll
             for (int e = e0; e < e0 + 4; e++) {
-              cur[t][e] = __builtin_amdgcn_exp2f(CT == GQ_I8_ROWS ? cur[t][e] - ms : __builtin_fmaf(cur[t][e], a.scale, -ms));
+              cur[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[t][e], a.scale, -ms));
               l += cur[t][e];
-            }
-            if constexpr (CT == GQ_I8_ROWS) {
-              const float4 d = lld<float4>(smem, sat + (32 * t + 2 * e0) * 4);
-              cur[t][e0] *= d.x, cur[t][e0 + 1] *= d.y, cur[t][e0 + 2] *= d.z, cur[t][e0 + 3] *= d.w;
             }
             if (c & 1) {
               float x[8];
@@ -484,9 +542,9 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
           }
         }
         __builtin_amdgcn_sched_barrier(0);
-        stagek(min(b + 2, bl), b & 1), stagev(min(b + 1, bl), (b + 1) & 1);
-        loadk(min(b + 3, bl)), loads(min(b + 3, bl), 0);
-        loadv(min(b + 2, bl)), loads(min(b + 2, bl), 1);
+        stagek(min(b + 2, bl), b & 1, kr, sc), stagev(min(b + 1, bl), (b + 1) & 1, vr, sc);
+        loadk(min(b + 3, bl), kr), loads(min(b + 3, bl), 0, sc);
+        loadv(min(b + 2, bl), vr), loads(min(b + 2, bl), 1, sc);
         if (rescale) {
 #pragma unroll
           for (int d = 0; d < ND; d++)
@@ -505,11 +563,11 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         turn(b + 1);
         __syncthreads();
       };
-      for (int b = 0;;) {
+      for (int b = b0;;) {
         body(b, sa, sb);
-        if (++b >= nblk) break;
+        if (++b >= b1) break;
         body(b, sb, sa);
-        if (++b >= nblk) break;
+        if (++b >= b1) break;
       }
     }
   } else {
@@ -521,25 +579,26 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       softmax(buf, st);
       output(buf);
     };
-    auto load = [&](int b) { loadk(b), loads(b, 0), loadv(b), loads(b, 1); };
-    if (nblk > 0) {
-      load(0);
+    auto load = [&](int b) { loadk(b, kr), loads(b, 0, sc), loadv(b, vr), loads(b, 1, sc); };
+    auto stage = [&](int b, int buf) { stagek(b, buf, kr, sc), stagev(b, buf, vr, sc); };
+    if (b0 < b1) {
+      load(b0);
+      query();
       if constexpr (NB == 2) {
-        stagek(0, 0), stagev(0, 0);
-        load(min(1, bl));
+        stage(b0, b0 & 1);
+        load(min(b0 + 1, bl));
         __syncthreads();
-        for (int b = 0; b < nblk; b++) {
-          const int n = min(b + 1, bl);
-          stagek(n, (b + 1) & 1), stagev(n, (b + 1) & 1); /* last read before the barrier below */
+        for (int b = b0; b < b1; b++) {
+          stage(min(b + 1, bl), (b + 1) & 1); /* last read before the barrier below */
           load(min(b + 2, bl));
           compute(b, b & 1);
           turn(b + 1);
           __syncthreads();
         }
       } else {
-        for (int b = 0; b < nblk; b++) {
+        for (int b = b0; b < b1; b++) {
           __syncthreads(); /* the planes are free */
-          stagek(b, 0), stagev(b, 0);
+          stage(b, 0);
           __syncthreads();
           load(min(b + 1, bl));
           compute(b, 0);
@@ -563,46 +622,131 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     if (kh == 1) return;
     const float m1 = x[lane], mt = fmaxf(m, m1), ms = mt == -INFINITY ? 0.f : mt;
     const float s0 = __builtin_amdgcn_exp2f(m - ms), s1 = __builtin_amdgcn_exp2f(m1 - ms);
-    l = l * s0 + x[64 + lane] * s1;
+    l = l * s0 + x[64 + lane] * s1, m = mt;
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
       for (int e = 0; e < 16; e++) o[d][e] = o[d][e] * s0 + x[64 * (2 + 16 * d + e) + lane] * s1;
   }
-  if (!live) return;
-  const float inv = l == 0.f ? 0.f : 1.0f / l; /* nothing seen: zeros */
+  /* Lanes (r, 0) and (r, 1) trade halves of two runs of eight dims, so that each
+   * has one whole: dims 32 d + 16 c + 8 h .. + 7. */
+  const bool whole = bp.y == 1;
+  const float inv = !whole ? 1.0f : l == 0.f ? 0.f : 1.0f / l; /* nothing seen: zeros */
+  const size_t at = (size_t)(tl.row + tok) * a.os + (size_t)qh * HD;
+  const size_t pat = ((size_t)(tl.row + tok) * a.n_heads + qh) * a.nch + part;
 #pragma unroll
   for (int d = 0; d < ND; d++)
 #pragma unroll
-    for (int c = 0; c < 4; c++) { /* dims 32 d + 8 c + 4 h .. + 3 */
-      const size_t at = (size_t)(rn.x + t0 + tok) * a.os + (size_t)qh * HD + 32 * d + 8 * c + 4 * h;
-      const float y[4] = {o[d][4 * c] * inv, o[d][4 * c + 1] * inv, o[d][4 * c + 2] * inv, o[d][4 * c + 3] * inv};
-      if constexpr (XT == GQ_F32) gst<float4>((float *)a.out + at, make_float4(y[0], y[1], y[2], y[3]));
-      else gst<uint2>((uint16_t *)a.out + at, make_uint2(pgd_pack(y[0], y[1]), pgd_pack(y[2], y[3])));
+    for (int c = 0; c < 2; c++) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        y[e] = o[d][8 * c + e] * inv, y[4 + e] = o[d][8 * c + 4 + e] * inv;
+        swap_halves(y[e], y[4 + e]);
+      }
+      const int dim = 32 * d + 16 * c + 8 * h;
+      if (live) {
+        if (whole) pgd_store8<XT>(a.out, at + dim, y);
+        else pgd_store8<GQ_F32>(a.part_o, pat * HD + dim, y);
+      }
     }
+  if (live && !whole && h == 0) gst<float2>(a.part_ml + 2 * pat, make_float2(m, l));
 }
 
-template <int CT, int XT, int HD>
-int launch(const AttArgs &a, int n_cu, hipStream_t s) {
-  constexpr int RG = XT == GQ_F32 ? 4 : 8, KH = 8 / RG;
-  const int tpt = 32 * RG / a.G;
-  const long long tiles = a.b.n_tokens / tpt + std::min(a.b.n_seqs, a.b.n_tokens), blocks = tiles * a.c.n_kv;
-  if (blocks >= (1ll << 31)) return -4;
-  (void)n_cu;
-  hipLaunchKernelGGL((prompt_kernel<CT, XT, HD, RG, KH>), dim3((unsigned)blocks), dim3(kPThreads), 0, s, a);
+/* The parts of a row's keys, a workgroup per token: out = sum_c o_c 2^(m_c - M) /
+ * sum_c l_c 2^(m_c - M), four dims of a head a thread. */
+template <int XT, int HD>
+__global__ __launch_bounds__(256) void prompt_merge_kernel(AttArgs a, int tpt) {
+  const int row = blockIdx.x, s = __builtin_amdgcn_readfirstlane(pgd_seq_of(a.b, row));
+  if (s >= a.b.n_seqs) return;
+  const int2 rn = pgd_rows(a.b, s);
+  if (row < rn.x || row >= rn.x + rn.y) return;
+  const int parts = tile_blocks(a, gq_sld<int>(a.b.pos + s), min((row - rn.x) / tpt * tpt + tpt, rn.y) - 1).y;
+  if (parts <= 1) return; /* its one part has written the result */
+  for (int i = threadIdx.x; i < a.n_heads * (HD / 4); i += 256) {
+    const int qh = i / (HD / 4), dim = 4 * (i % (HD / 4));
+    const size_t at = ((size_t)row * a.n_heads + qh) * a.nch;
+    float M = -INFINITY;
+    for (int c = 0; c < parts; c++) M = fmaxf(M, gld<float>(a.part_ml + 2 * (at + c)));
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < parts; c++) {
+      const float2 ml = gld<float2>(a.part_ml + 2 * (at + c));
+      const float4 o = gld<float4>(a.part_o + (at + c) * HD + dim);
+      const float w = __builtin_amdgcn_exp2f(ml.x - ms);
+      L = __builtin_fmaf(ml.y, w, L);
+      y.x = __builtin_fmaf(o.x, w, y.x), y.y = __builtin_fmaf(o.y, w, y.y);
+      y.z = __builtin_fmaf(o.z, w, y.z), y.w = __builtin_fmaf(o.w, w, y.w);
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    const size_t o = (size_t)row * a.os + (size_t)qh * HD + dim;
+    if constexpr (XT == GQ_F32) gst<float4>((float *)a.out + o, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+    else gst<uint2>((uint16_t *)a.out + o, make_uint2(pgd_pack(y.x * inv, y.y * inv), pgd_pack(y.z * inv, y.w * inv)));
+  }
+}
+
+template <int CT, int XT, int HD, int RG>
+int launch(const AttArgs &a, unsigned blocks, int tpt, hipStream_t s) {
+  hipLaunchKernelGGL((prompt_kernel<CT, XT, HD, RG, 8 / RG>), dim3(blocks), dim3(kPThreads), 0, s, a);
+  if (a.nch > 1) hipLaunchKernelGGL((prompt_merge_kernel<XT, HD>), dim3(a.b.n_tokens), dim3(256), 0, s, a, tpt);
   return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
 template <int CT, int XT>
-int launch_hd(const AttArgs &a, int hd, int n_cu, hipStream_t s) {
-  return hd == 64 ? launch<CT, XT, 64>(a, n_cu, s) : launch<CT, XT, 128>(a, n_cu, s);
+int launch_hd(const AttArgs &a, int hd, const PromptShape &f, hipStream_t s) {
+  const int tpt = f.rows / a.G;
+  if constexpr (XT == GQ_BF16)
+    if (f.rows == 256) return hd == 64 ? launch<CT, XT, 64, 8>(a, f.blocks, tpt, s) : launch<CT, XT, 128, 8>(a, f.blocks, tpt, s);
+  return hd == 64 ? launch<CT, XT, 64, 4>(a, f.blocks, tpt, s) : launch<CT, XT, 128, 4>(a, f.blocks, tpt, s);
 }
 
 } // namespace
 
-int gq_launch_paged_prompt(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu, hipStream_t s) {
-  const bool f = xtype == GQ_F32;
-  if (cache == GQ_F32) return f ? launch_hd<GQ_F32, GQ_F32>(a, head_dim, n_cu, s) : launch_hd<GQ_F32, GQ_BF16>(a, head_dim, n_cu, s);
-  if (cache == GQ_BF16) return f ? launch_hd<GQ_BF16, GQ_F32>(a, head_dim, n_cu, s) : launch_hd<GQ_BF16, GQ_BF16>(a, head_dim, n_cu, s);
-  return f ? launch_hd<GQ_I8_ROWS, GQ_F32>(a, head_dim, n_cu, s) : launch_hd<GQ_I8_ROWS, GQ_BF16>(a, head_dim, n_cu, s);
+/* The launch: rows of a tile (256, or 128 where those leave CUs idle; fp32
+ * queries always 128) and parts of a tile's keys, whichever should take least.
+ * Microseconds: a workgroup, `fix` and `tau` a block of 64 keys; more of them
+ * than CUs, their sum and a quarter of the longest for what the last ones leave
+ * idle; parts, their merge.  Of the lengths the host knows the longest and the
+ * number of new tokens alone, and takes the sequences for equally long.
+ *
+ * tau: one tile of 64 tokens over 8192 positions (32 heads over 8).  The other
+ * constants are fitted to 300 launches timed with every choice (1 to 8
+ * sequences, 1 to 2000 new tokens at 0 to 8000, head groups of 1 to 8): the rule's
+ * choices take 2.5% more than the best ones together, 7% more for the worst in
+ * ten; one part and 256 rows always, up to five times as long. */
+PromptShape gq_paged_prompt_shape(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu) {
+  const bool f = xtype == GQ_F32, wide = head_dim > 64;
+  const int t = cache == GQ_F32 ? 0 : cache == GQ_BF16 ? 1 : 2;
+  constexpr double kTau[2][3][3] = {{{1.31, 1.29, 1.35}, {0.94, 0.92, 0.95}, {2.42, 1.53, 1.80}},  /* head_dim 64: bf16 queries in 256 and 128 rows, fp32 */
+                                    {{1.98, 1.80, 1.90}, {1.58, 1.31, 1.40}, {5.66, 3.26, 3.39}}}; /* 128 */
+  const double fix = (f ? 5.0 : 10.0) * (wide ? 1.0 : 0.3);
+  const int seqs = std::min(a.b.n_seqs, a.b.n_tokens), each = (a.b.n_tokens + seqs - 1) / seqs;
+  const int nblk = std::max(1, (a.b.max_len + kKeys - 1) / kKeys);
+  const double mean = std::min((double)nblk, (std::max(0, a.b.max_len - each) + 0.5 * each) / kKeys + 1);
+  PromptShape best{};
+  double us = 1e30;
+  for (int rows = f ? 128 : 256; rows >= 128; rows /= 2) {
+    const int tpt = rows / a.G;
+    const double w = (double)seqs * ((each + tpt - 1) / tpt) * a.c.n_kv, tau = kTau[wide][f ? 2 : rows == 128][t];
+    for (int k = 1; k <= std::min(16, nblk); k++) {
+      const int span = (nblk + k - 1) / k;
+      const double parts = std::max(1.0, mean / span), longest = fix + tau * span;
+      const double load = w * (parts * fix + tau * mean) / n_cu;
+      double c = w * parts <= n_cu ? longest : std::max(longest, load + longest / 4);
+      if (k > 1) c += 4 + 2e-6 * a.b.n_tokens * a.n_heads * head_dim * k;
+      if (c < us) us = c, best.rows = rows, best.span = span, best.parts = (nblk + span - 1) / span;
+    }
+  }
+  const long long tiles = a.b.n_tokens / (best.rows / a.G) + seqs, blocks = tiles * a.c.n_kv * best.parts;
+  best.blocks = blocks < (1ll << 31) ? (unsigned)blocks : 0u;
+  return best;
+}
+
+int gq_launch_paged_prompt(const AttArgs &a, int cache, int xtype, int head_dim, const PromptShape &f, hipStream_t s) {
+  const bool x = xtype == GQ_F32;
+  if (cache == GQ_F32) return x ? launch_hd<GQ_F32, GQ_F32>(a, head_dim, f, s) : launch_hd<GQ_F32, GQ_BF16>(a, head_dim, f, s);
+  if (cache == GQ_BF16) return x ? launch_hd<GQ_BF16, GQ_F32>(a, head_dim, f, s) : launch_hd<GQ_BF16, GQ_BF16>(a, head_dim, f, s);
+  return x ? launch_hd<GQ_I8_ROWS, GQ_F32>(a, head_dim, f, s) : launch_hd<GQ_I8_ROWS, GQ_BF16>(a, head_dim, f, s);
 }

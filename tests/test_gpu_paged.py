@@ -15,7 +15,8 @@ step), M = sum p |v| / sum p and S = the largest sum |q k| / sqrt(hd):
     bar of the single-sequence attention.
   bf16 rows: the result's rounding w |y|, beside that.
   bf16 prompts: every probability rounded to bf16 besides: w M; and over an fp32
-    cache K's and V's values too, 2 w S M and w M.
+    or int8 cache K's and V's values too: scores off by w S, probabilities by
+    twice that relative to their sum, 2 w S M, and w M from V.
 """
 import numpy as np
 import pytest
@@ -168,7 +169,7 @@ def check_attention(w, q, got, rows, xt, prompt):
             tol = tol + W * np.abs(y)
             if prompt:
                 tol = tol + W * mag
-                if w.cache == F32:
+                if w.cache != BF16:
                     tol = tol + (2 * W * top + W) * mag
         off = np.abs(got[t].reshape(nh, hd) - y)
         assert np.isfinite(got[t]).all(), (t, w.at[t])
