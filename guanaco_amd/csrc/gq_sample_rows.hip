@@ -25,6 +25,7 @@
  */
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "gq_device.h"
 #include "gq_internal.h"
@@ -37,8 +38,9 @@ constexpr int kTopT = 256, kTop = 4096;        /* threads and tokens of a workgr
 constexpr int kBins = 512, kLast = kBins - 2;  /* a part's histogram; min_p moves what it leaves out one bin on */
 constexpr int kFine = 2048;                    /* bins of eleven bits */
 constexpr int kChunks = 16;
-constexpr int kList = 8192;                    /* tokens of the border's bin that fit LDS */
-constexpr int kRows = 4096;                    /* rows a launch: 28 MB of workspace at most */
+constexpr int kShare = 512;                    /* tokens of the border's bin that a wave can list */
+constexpr int kList = kW * kShare;
+constexpr int kRows = 512;                     /* rows a launch: 40 MB of workspace at most */
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -50,6 +52,14 @@ struct Part { /* what a part of a row leaves for the last launch */
   int pad;
 };
 
+struct Border { /* of a row, by the third launch */
+  unsigned long long mass[kBins]; /* of the whole row */
+  unsigned long long base, ahead; /* before the border's bin: the count (top-k) or mass, and the mass */
+  int bin, from; /* bins from .. bin are listed */
+  int pass;
+  int pad;
+};
+
 struct SampArgs {
   const float *x;
   const float *temperature, *top_p, *min_p, *rnd;
@@ -58,7 +68,11 @@ struct SampArgs {
   float *logprobs;
   uint64_t *tops;
   Part *parts;
+  Border *borders;
+  uint64_t *lists; /* [row][lister][kList] */
+  int *counts;     /* [row][lister]: -1, if they did not fit */
   int vocab, n_tops, chunks, chunk; /* chunk: tokens a part, a multiple of 4 */
+  int listers;                      /* workgroups a row of the third launch */
   long long stride;
   int S; /* w is held in units of 2^-S */
 };
@@ -83,53 +97,71 @@ __device__ __forceinline__ T wave_reduce(T v, F f) {
   for (int o = 32; o; o >>= 1) v = f(v, (T)__shfl_xor(v, o, 64));
   return v;
 }
-__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {
-  return wave_reduce(v, [](unsigned long long a, unsigned long long b) { return a + b; });
+/* running sums over the lanes: within rows of 16 by row_shr 1, 2, 4 and 8, then
+ * row 0's and 2's last to the row behind, then the second row's to the last two */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_add(unsigned long long v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((unsigned long long)(uint32_t)hi << 32 | (uint32_t)lo);
 }
 __device__ __forceinline__ unsigned long long wave_scan(unsigned long long v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  return v;
+  v = dpp_add<0x111, 0xf>(v), v = dpp_add<0x112, 0xf>(v), v = dpp_add<0x114, 0xf>(v), v = dpp_add<0x118, 0xf>(v);
+  return dpp_add<0x143, 0xc>(dpp_add<0x142, 0xa>(v));
 }
+__device__ __forceinline__ unsigned long long last_lane(unsigned long long v) {
+  return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) { return last_lane(wave_scan(v)); }
 
-/* f(v, i) for the tokens i of [lo, hi) in some order: four neighbours a thread
- * at a time, U such loads in flight; lo is a multiple of 4 */
-template <int U, class F>
-__device__ __forceinline__ void tokens(const float *x, int lo, int hi, int threads, int tid, F f) {
+/* use(f(v, i)) for the tokens i of [lo, hi) in some order: four neighbours a
+ * thread at a time, U such loads in flight, their f side by side; lo is a
+ * multiple of 4 */
+template <int U, class F, class G>
+__device__ __forceinline__ void tokens(const float *x, int lo, int hi, int threads, int tid, F f, G use) {
   int i = lo + 4 * tid;
   for (; i + 4 * (U - 1) * threads + 3 < hi; i += 4 * U * threads) {
     f32x4u v[U];
 #pragma unroll
     for (int u = 0; u < U; u++) v[u] = *(const f32x4u *)(x + i + 4 * u * threads);
+    decltype(f(0.f, 0)) r[4 * U];
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int u = 0; u < 4 * U; u++) r[u] = f(v[u / 4][u & 3], i + 4 * (u / 4) * threads + (u & 3));
 #pragma unroll
-      for (int e = 0; e < 4; e++) f(v[u][e], i + 4 * u * threads + e);
+    for (int u = 0; u < 4 * U; u++) use(r[u]);
   }
   for (; i < hi; i += 4 * threads) {
     if (i + 3 < hi) {
       const f32x4u v = *(const f32x4u *)(x + i);
 #pragma unroll
-      for (int e = 0; e < 4; e++) f(v[e], i + e);
+      for (int e = 0; e < 4; e++) use(f(v[e], i + e));
     } else {
-      for (int e = i; e < hi; e++) f(x[e], e);
+      for (int e = i; e < hi; e++) use(f(x[e], e));
     }
   }
 }
+template <int U, class F>
+__device__ __forceinline__ void tokens(const float *x, int lo, int hi, int threads, int tid, F f) {
+  struct None {};
+  tokens<U>(x, lo, hi, threads, tid, [&](float v, int i) { return f(v, i), None{}; }, [](None) {});
+}
 
-/* 2^(i / 64) to tab, by the first wave */
-__device__ __forceinline__ void table(double *tab) {
-  if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x / 64);
+/* 2^(S + i / 64) to tab, by the first wave */
+__device__ __forceinline__ void table(double *tab, int S) {
+  if (threadIdx.x < 64) tab[threadIdx.x] = __builtin_ldexp(exp2((double)threadIdx.x / 64), S);
+}
+/* a b + c with c in scalar registers: the compiler copies it to others first */
+__device__ __forceinline__ double fma_s(double a, double b, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+  return d;
 }
 
 /* a row's parameters and what follows from them alone */
 struct Row {
   float top, T, min_p, scale;
-  int k, S;
+  int k;
   bool inf, by_k, by_p;
   float p;
   double c;   /* e^((v - top) / T) = 2^((v - top) c / 64) */
@@ -147,35 +179,39 @@ struct Row {
     top = value_of((uint32_t)(first >> 32));
     inf = top == INFINITY; /* such a row's infinities weigh 1, the others nothing */
     if (inf) top = 0.f;
-    S = a.S;
     c = 92.332482616893656877 / (double)T; /* 64 / ln 2 */
     low = min_p > 0.f ? 64.0 * log2((double)min_p) : -INFINITY;
     /* the last bin takes what weighs nothing in units of 2^-S */
-    scale = (float)(kLast / ((a.S + 1.5) * 0.6931471805599453)) / T;
+    scale = fminf((float)(kLast / ((a.S + 1.5) * 0.6931471805599453)) / T, 3e38f);
   }
   __device__ float see(float v) const { return inf ? (v == INFINITY ? 0.f : -INFINITY) : v; }
   __device__ double y(float v) const { return ((double)v - (double)top) * c; }
   __device__ bool passes(float v) const { return y(v) >= low; }
   /* bins in descending order of the logits, none of which mixes what min_p
    * keeps with what it does not: that goes one bin on */
-  __device__ int bin(float v) const {
-    const int b = v == top ? 0 : (int)fminf((top - v) * scale, (float)kLast);
-    return min_p > 0.f && !passes(v) ? b + 1 : b;
+  __device__ int bin0(float v) const { return (int)fminf((top - v) * scale, (float)kLast); }
+  __device__ int bin(float v) const { return bin0(v) + (min_p > 0.f && !passes(v)); }
+  /* logits between which all of bins b0 .. b1 lie, and some others: the bin's
+   * arithmetic is off by 2^-22 of (top - v) and of top at most */
+  __device__ void bounds(int b0, int b1, float &lo, float &hi) const {
+    const float d1 = (float)(b1 + 1) / scale, d0 = (float)(b0 - 1) / scale, more = 1e-6f * fabsf(top) + 1e-43f;
+    hi = top;
+    lo = b1 < kLast && d1 < 1e38f ? fmaxf(top - d1 * 1.000001f - more, -3.402823466e38f) : -3.402823466e38f;
+    if (b0 > 1 && d0 < 1e38f) hi = fminf(top - d0 * 0.999999f + more, top);
   }
   /* e^((v - top) / T) in units of 2^-S, nearest even.  2^((k + f) / 64): 2^(k /
    * 64) from the table, e^(f ln 2 / 64) by its series to the fifth power (the
    * next term is below 2^-54), and 2^52 added: the low bits are the number. */
   __device__ unsigned long long mass(float v) const {
-    const double t = fmax(y(v), -4096.0); /* 2^-64 is nothing */
-    const double n = __builtin_rint(t), f = t - n;
-    double s = __builtin_fma(f, 0x1.5d87fe78a6731p-40 /* (ln 2 / 64)^5 / 120 */, 0x1.3b2ab6fba4e77p-31);
-    s = __builtin_fma(f, s, 0x1.c6b08d704a0c0p-23);
-    s = __builtin_fma(f, s, 0x1.ebfbdff82c58fp-15);
-    s = __builtin_fma(f, s, 0x1.62e42fefa39efp-7);
-    const int i = (int)n;
-    const double b = tab[i & 63];
-    s = __builtin_ldexp(__builtin_fma(b * f, s, b), (i >> 6) + S);
-    return __builtin_bit_cast(unsigned long long, s + 0x1p52) & 0xfffffffffffffull;
+    const double t = fmax(y(v), -4096.0), n = t + 0x1.8p52, f = t - (n - 0x1.8p52); /* 2^-64 is nothing */
+    double s = fma_s(f, 0x1.5d87fe78a6731p-40 /* (ln 2 / 64)^5 / 120 */, 0x1.3b2ab6fba4e77p-31);
+    s = fma_s(f, s, 0x1.c6b08d704a0c0p-23);
+    s = fma_s(f, s, 0x1.ebfbdff82c58fp-15);
+    s = fma_s(f, s, 0x1.62e42fefa39efp-7);
+    const int i = (int)__builtin_bit_cast(uint64_t, n);
+    const uint64_t e = __builtin_bit_cast(uint64_t, tab[i & 63]);
+    const double b = __builtin_bit_cast(double, e + ((uint64_t)(uint32_t)((i >> 6) << 20) << 32));
+    return __builtin_bit_cast(unsigned long long, __builtin_fma(b * f, s, b) + 0x1p52) & 0xfffffffffffffull;
   }
 };
 
@@ -213,7 +249,7 @@ __device__ __forceinline__ uint64_t first_of(const SampArgs &a, long long row, u
 }
 
 /* the histogram of a part of a row, or only the sum of what it keeps */
-__global__ __launch_bounds__(kT) void parts_kernel(SampArgs a) {
+__global__ __launch_bounds__(kT, 8) void parts_kernel(SampArgs a) {
   __shared__ double tab[64];
   __shared__ uint64_t first;
   __shared__ unsigned long long mass[kBins], kept;
@@ -221,7 +257,7 @@ __global__ __launch_bounds__(kT) void parts_kernel(SampArgs a) {
   __shared__ int pass;
   const int tid = threadIdx.x;
   const long long r = blockIdx.y;
-  table(tab);
+  table(tab, a.S);
   for (int i = tid; i < kBins; i += kT) mass[i] = 0, cnt[i] = 0;
   if (tid == 0) kept = 0, pass = -1;
   const uint64_t f = first_of(a, r, &first);
@@ -234,7 +270,8 @@ __global__ __launch_bounds__(kT) void parts_kernel(SampArgs a) {
     unsigned long long s = 0;
     tokens<2>(x, lo, hi, kT, tid, [&](float v, int) {
       v = row.see(v);
-      if (row.min_p == 0.f || row.passes(v)) s += row.mass(v);
+      const unsigned long long m = row.mass(v);
+      s += row.passes(v) ? m : 0;
     });
     s = wave_sum(s);
     if ((tid & 63) == 0) atomicAdd(&kept, s);
@@ -243,14 +280,30 @@ __global__ __launch_bounds__(kT) void parts_kernel(SampArgs a) {
     return;
   }
   int last = -1;
-  tokens<2>(x, lo, hi, kT, tid, [&](float v, int) {
-    v = row.see(v);
-    if (!(v > -INFINITY)) return;
-    const int b = row.bin(v);
-    if (row.min_p > 0.f && b > last && row.passes(v)) last = b;
-    atomicAdd(&mass[b], row.mass(v));
-    if (row.by_k) atomicAdd(&cnt[b], 1u);
-  });
+  struct Token {
+    unsigned long long m;
+    int b;
+  };
+  const auto fill = [&](auto min_p, auto count) {
+    tokens<1>(
+        x, lo, hi, kT, tid,
+        [&](float v, int) {
+          v = row.see(v);
+          const bool in = !min_p || row.passes(v);
+          const int b = row.bin0(v) + !in;
+          if (min_p) last = max(last, in ? b : -1);
+          return Token{row.mass(v), v > -INFINITY ? b : -1};
+        },
+        [&](Token t) {
+          if (t.b < 0) return;
+          atomicAdd(&mass[t.b], t.m);
+          if (count) atomicAdd(&cnt[t.b], 1u);
+        });
+  };
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
+  if (row.min_p > 0.f) row.by_k ? fill(yes, yes) : fill(yes, no);
+  else row.by_k ? fill(no, yes) : fill(no, no);
   if (last >= 0) atomicMax(&pass, last);
   __syncthreads();
   for (int i = tid; i < kBins; i += kT) to.mass[i] = mass[i], to.cnt[i] = cnt[i];
@@ -274,6 +327,7 @@ __device__ unsigned long long block_sum(Shared &sh, unsigned long long s) {
   if ((threadIdx.x & 63) == 0) sh.wsum[threadIdx.x >> 6] = s;
   __syncthreads();
   s = 0;
+#pragma unroll
   for (int w = 0; w < kW; w++) s += sh.wsum[w];
   __syncthreads();
   return s;
@@ -290,7 +344,8 @@ __device__ void find_bin(Shared &sh, bool count, unsigned long long base, double
   if (lane == 63) sh.wsum[wave] = s;
   __syncthreads();
   unsigned long long off = base;
-  for (int w = 0; w < wave; w++) off += sh.wsum[w];
+#pragma unroll
+  for (int w = 0; w < kW - 1; w++) off += w < wave ? sh.wsum[w] : 0;
   const unsigned long long c0 = off + s - a - b, c1 = c0 + a, c2 = c1 + b;
   if (!((double)c0 >= target) || tid == 0) {
     const int at = (double)c1 >= target ? 2 * tid : (double)c2 >= target || tid == kT - 1 ? 2 * tid + 1 : -1;
@@ -299,13 +354,130 @@ __device__ void find_bin(Shared &sh, bool count, unsigned long long base, double
   __syncthreads();
 }
 
+/* tokens i .. i + 3, those before `to` */
+__device__ __forceinline__ f32x4u four(const float *x, int i, int to) {
+  if (i + 3 < to) return *(const f32x4u *)(x + i);
+  f32x4u v;
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = i + e < to ? x[i + e] : -INFINITY;
+  return v;
+}
+
+/* The tokens lo .. hi - 1 (lo a multiple of 4) of bins b0 .. b1, and a few of
+ * the next ones, to each wave's own share of a list; returns how many a wave
+ * has, of which the first kShare are listed.  Two compares a token: what a
+ * workgroup reads bounds it (10 us for 513 KB by one of them). */
+template <int U>
+__device__ __forceinline__ int list_tokens(const Row &row, const float *x, int lo, int hi, int b0, int b1, uint64_t *list) {
+  constexpr int D = 4 * kT;
+  float vlo, vhi;
+  row.bounds(b0, b1, vlo, vhi);
+  int n = 0;
+  for (int b = lo; b < hi; b += U * D) {
+    const int i = b + 4 * threadIdx.x;
+    f32x4u v[U];
+    if (b + U * D <= hi) {
+#pragma unroll
+      for (int u = 0; u < U; u++) v[u] = *(const f32x4u *)(x + i + u * D);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++) v[u] = four(x, i + u * D, hi);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      uint64_t hit[4], any = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (row.inf) v[u][e] = row.see(v[u][e]);
+        hit[e] = __ballot(v[u][e] >= vlo && v[u][e] <= vhi), any |= hit[e];
+      }
+      if (any)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int j = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(hit[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[e], 0));
+          if (v[u][e] >= vlo && v[u][e] <= vhi && j < kShare) list[j] = comp_of(v[u][e], i + u * D + e);
+          n += __builtin_popcountll(hit[e]);
+        }
+    }
+  }
+  return n;
+}
+
+/* a row's border of top-k, or else of top-p: its bin, and the tokens of it
+ * among the parts that a workgroup looks through */
+__global__ __launch_bounds__(kT) void list_kernel(SampArgs a) {
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long long r = blockIdx.y;
+  const Part *parts = a.parts + r * a.chunks;
+  const uint64_t first = first_of(a, r, &sh.first);
+  const Row row(a, r, first, sh.tab);
+  if (!first || !(row.T > 0.f) || !(row.by_k || row.by_p)) return;
+  /* the histogram of the whole row */
+  unsigned long long m0 = 0;
+  uint32_t c0 = 0;
+  const int end = a.chunks - 1;
+  if (tid < kBins) {
+    unsigned long long m[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) m[c] = parts[min(c, end)].mass[tid];
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) m0 += c <= end ? m[c] : 0;
+  } else if (row.by_k) {
+    uint32_t m[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) m[c] = parts[min(c, end)].cnt[tid - kBins];
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) c0 += c <= end ? m[c] : 0;
+  }
+  static_assert(kT == 2 * kBins && kFine == 2 * kT, "a bin is two threads'");
+  if (tid < kBins) sh.mass[tid] = m0, sh.mass[tid + kBins] = 0;
+  else sh.cnt[tid - kBins] = c0, sh.cnt[tid] = 0;
+  sh.mass[tid + kT] = 0, sh.cnt[tid + kT] = 0;
+  __syncthreads();
+  const double target = row.by_k ? (double)row.k : (double)row.p * (double)block_sum(sh, m0);
+  find_bin(sh, row.by_k, 0, target);
+  const unsigned long long base = sh.before;
+  /* a bin of mass 0: what is left weighs nothing.  With top-p to come, the
+   * bins before top-k's border too, if they fit: top-p's is among them */
+  const int bin = sh.in ? sh.at : kBins;
+  const int from = bin < kBins && row.by_k && row.by_p && base + sh.n <= kList / 2 ? 0 : bin;
+  const unsigned long long ahead = block_sum(sh, tid < bin ? m0 : 0);
+  Border &to = a.borders[r];
+  if (blockIdx.x == 0) {
+    if (tid < kBins) to.mass[tid] = m0;
+    if (wave == 0) {
+      int pass = row.min_p > 0.f && lane < a.chunks ? parts[lane].pass : -1;
+      pass = wave_reduce(pass, [](int p, int q) { return max(p, q); });
+      if (lane == 0) to.base = base, to.ahead = ahead, to.bin = bin, to.from = from, to.pass = pass;
+    }
+  }
+  int n = 0;
+  const int per = (a.chunks + a.listers - 1) / a.listers * a.chunk;
+  const int lo = min(a.vocab, (int)blockIdx.x * per), hi = min(a.vocab, lo + per);
+  if (bin < kBins) n = list_tokens<8>(row, a.x + r * a.stride, lo, hi, from, bin, sh.list + wave * kShare);
+  if (lane == 0) sh.wsum[wave] = n;
+  __syncthreads();
+  int at = 0, all = 0;
+  bool fits = true;
+#pragma unroll
+  for (int w = 0; w < kW; w++) {
+    const int m = (int)sh.wsum[w];
+    at += w < wave ? m : 0, all += m, fits = fits && m <= kShare;
+  }
+  const long long l = r * a.listers + blockIdx.x;
+  if (tid == 0) a.counts[l] = fits ? all : -1;
+  if (fits)
+    for (int j = lane; j < n; j += GQ_WAVE) a.lists[l * kList + at + j] = sh.list[wave * kShare + j];
+}
+
 __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = a.vocab;
   const long long r = blockIdx.x;
   const float *x = a.x + r * a.stride;
   const Part *parts = a.parts + r * a.chunks;
-  table(sh.tab);
+  table(sh.tab, a.S);
   const uint64_t first = first_of(a, r, &sh.first);
   const Row row(a, r, first, sh.tab);
   if (!first || !(row.T > 0.f)) { /* nothing to pick, or greedy */
@@ -317,94 +489,91 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   }
   int border = kBins, pass = row.min_p > 0.f ? -1 : kBins;
   uint64_t cut = 0; /* tokens with a smaller (logit, index) are left out */
-  /* the listed logits: keys klo .. khi */
-  uint32_t klo = 1, khi = 0, n = 0;
+  /* the tokens of bins b0 .. b1 (and a few of the next ones), if they fit LDS:
+   * every wave's own share of them */
+  int b0 = 1, b1 = 0, n = 0;
   bool listed = false;
-  /* the lowest key of bins 0 .. b: a search of 64 keys at a time */
-  const auto lowest = [&](int b) {
-    uint32_t lo = key_of(-3.402823466e38f), hi = key_of(row.top);
-    while (lo < hi) {
-      const uint32_t step = (hi - lo) / 64 + 1;
-      const uint64_t u = (uint64_t)lo + (uint64_t)lane * step;
-      const uint64_t in = __ballot(u >= hi || row.bin(value_of((uint32_t)u)) <= b);
-      const int f = in ? __builtin_ctzll(in) : 64;
-      const uint64_t up = (uint64_t)lo + (uint64_t)f * step;
-      if (f) lo = lo + (uint32_t)(f - 1) * step + 1;
-      hi = f == 0 ? lo : (uint32_t)min(up, (uint64_t)hi);
-    }
-    return hi;
-  };
-  /* the tokens of bins b0 .. b1 to the list, if they fit */
-  const auto gather = [&](int b0, int b1) {
-    khi = b0 ? lowest(b0 - 1) - 1 : key_of(row.top), klo = lowest(b1);
-    const float vlo = value_of(klo), vhi = value_of(khi);
-    __syncthreads();
+  const uint64_t *list = sh.list;
+  const auto gather = [&](int bin) {
+    b0 = b1 = bin, list = sh.list + wave * kShare;
+    n = list_tokens<2>(row, x, 0, V, bin, bin, sh.list + wave * kShare);
     if (tid == 0) sh.n = 0;
     __syncthreads();
-    const auto put = [&](float v, int i) {
-      v = row.see(v);
-      if (v >= vlo && v <= vhi) {
-        const uint32_t j = atomicAdd(&sh.n, 1u);
-        if (j < (uint32_t)kList) sh.list[j] = comp_of(v, i);
-      }
-    };
-    tokens<4>(x, 0, V, kT, tid, put);
+    if (lane == 0 && n > kShare) sh.n = 1;
     __syncthreads();
-    n = sh.n, listed = n <= (uint32_t)kList;
+    listed = !sh.n;
     __syncthreads();
   };
-  /* f(comp) for the kept ones of the listed tokens with c0 <= comp <= c1 */
-  const auto each = [&](uint64_t c0, uint64_t c1, auto f) {
+  /* f(v, comp) for the tokens of a bin with comp >= cut */
+  const auto each = [&](int bin, auto f) {
     if (listed) {
-      for (uint32_t j = tid; j < n; j += kT) {
-        const uint64_t c = sh.list[j];
-        if (c >= c0 && c <= c1) f(c);
+      for (int j = lane; j < n; j += GQ_WAVE) {
+        const uint64_t c = list[j];
+        const float v = value_of((uint32_t)(c >> 32));
+        if (c >= cut && row.bin(v) == bin) f(v, c);
       }
     } else {
+      float vlo, vhi;
+      row.bounds(bin, bin, vlo, vhi);
       tokens<1>(x, 0, V, kT, tid, [&](float v, int i) {
         v = row.see(v);
+        if (!(v >= vlo && v <= vhi)) return;
         const uint64_t c = comp_of(v, i);
-        if (v > -INFINITY && c >= c0 && c <= c1) f(c);
+        if (c >= cut && row.bin(v) == bin) f(v, c);
       });
     }
   };
   if (row.by_k || row.by_p) {
-    /* bin t of the whole row is thread t's */
-    unsigned long long m0 = 0, c0 = 0;
-    if (tid < kBins) {
-      for (int c = 0; c < a.chunks; c++) m0 += parts[c].mass[tid];
-      if (row.by_k)
-        for (int c = 0; c < a.chunks; c++) c0 += parts[c].cnt[tid];
-    }
-    if (row.min_p > 0.f)
-      for (int c = 0; c < a.chunks; c++) pass = max(pass, parts[c].pass);
-    for (int i = tid; i < kFine; i += kT) sh.mass[i] = i < kBins ? m0 : 0, sh.cnt[i] = i < kBins ? (uint32_t)c0 : 0;
-    __syncthreads();
-    unsigned long long whole = 0; /* mass of what top-k keeps */
-    for (int by = 0; by < 2; by++) {
-      const bool count = by == 0;
-      if (count ? !row.by_k : !row.by_p) {
-        if (count) whole = block_sum(sh, m0);
-        continue;
+    const Border &bd = a.borders[r];
+    const unsigned long long m0 = tid < kBins ? bd.mass[tid] : 0; /* bin t is thread t's */
+    if (row.min_p > 0.f) pass = bd.pass;
+    { /* the third launch's lists, one behind the other */
+      const int m = lane < a.listers ? a.counts[r * a.listers + lane] : 0;
+      listed = !__ballot(m < 0);
+      int sum = listed ? m : 0;
+#pragma unroll
+      for (int o = 1; o < kChunks; o <<= 1) {
+        const int u = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += u;
       }
+      const int all = __builtin_amdgcn_readlane(sum, kChunks - 1);
+      listed = listed && all <= kList;
+      if (listed) {
+        for (int l = 0; l < a.listers; l++) {
+          const int from = l ? __builtin_amdgcn_readlane(sum, l - 1) : 0, k = __builtin_amdgcn_readlane(m, l);
+          for (int j = tid; j < k; j += kT) sh.list[from + j] = a.lists[(r * a.listers + l) * kList + j];
+        }
+        const int share = (all + kW - 1) / kW, at = min(all, wave * share);
+        list = sh.list + at, n = min(all - at, share);
+        b0 = bd.from, b1 = bd.bin;
+      }
+      __syncthreads();
+    }
+    unsigned long long whole = 0; /* mass of what top-k keeps */
+    if (!row.by_k) whole = block_sum(sh, m0);
+    for (int by = row.by_k ? 0 : 1; by < (row.by_p ? 2 : 1); by++) {
+      const bool count = by == 0;
       const double target = count ? (double)row.k : (double)row.p * (double)whole;
-      find_bin(sh, count, 0, target);
-      const int bin = sh.at;
-      unsigned long long base = sh.before, in = sh.in; /* count or mass before the border's bin, its own mass */
-      const uint32_t below = sh.n;
-      const unsigned long long ahead = count ? block_sum(sh, tid < bin ? m0 : 0) : 0;
-      unsigned long long above = ahead; /* mass before it */
-      if (in == 0) { /* what is left weighs nothing */
+      int bin = bd.bin;
+      unsigned long long base = bd.base; /* count or mass before the border's bin */
+      if (!count && row.by_k) { /* the histogram of what top-k keeps */
+        for (int i = tid; i < kFine; i += kT) sh.mass[i] = i < border ? m0 : i == border ? whole - bd.ahead : 0;
+        __syncthreads();
+        find_bin(sh, false, 0, target);
+        bin = sh.at, base = sh.before;
+      }
+      unsigned long long above = bd.ahead, in = 0; /* mass before it; of the border itself */
+      if (count && bin == kBins) { /* what is left weighs nothing */
         whole = above;
         continue;
       }
-      /* the bins before it too, if they fit: top-p looks among them next */
-      const uint32_t lo = lowest(bin), hi = bin ? lowest(bin - 1) - 1 : key_of(row.top);
-      if (!listed || lo < klo || hi > khi) gather(count && row.by_p && base + below <= (uint64_t)kList ? 0 : bin, bin);
-      const uint64_t lo64 = max(cut, (uint64_t)lo << 32), hi64 = (uint64_t)hi << 32 | 0xffffffffu;
+      if (!listed || bin < b0 || bin > b1) gather(bin);
       /* eleven bits of (logit, index) at a time, after those that all share */
-      int shift = lo == hi ? 32 : 64 - __builtin_clz(lo ^ hi);
-      uint64_t prefix = shift < 64 ? lo64 >> shift : 0;
+      float vlo, vhi;
+      row.bounds(bin, bin, vlo, vhi);
+      const uint32_t klo = key_of(vlo), khi = key_of(vhi);
+      int shift = klo == khi ? 32 : 64 - __builtin_clz(klo ^ khi);
+      uint64_t prefix = shift < 64 ? ((uint64_t)klo << 32) >> shift : 0;
       uint32_t left = 2;
       while (left > 1 && shift > 0) {
         const int bits = min(11, shift), mask = (1 << bits) - 1;
@@ -412,11 +581,11 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
         __syncthreads();
         for (int i = tid; i < kFine; i += kT) sh.cnt[i] = 0, sh.mass[i] = 0;
         __syncthreads();
-        each(lo64, hi64, [&](uint64_t c) {
+        each(bin, [&](float v, uint64_t c) {
           if (shift + bits < 64 && c >> (shift + bits) != prefix) return;
           const int d = mask - ((int)(c >> shift) & mask); /* the largest first */
           atomicAdd(&sh.cnt[d], 1u);
-          atomicAdd(&sh.mass[d], row.mass(value_of((uint32_t)(c >> 32))));
+          atomicAdd(&sh.mass[d], row.mass(v));
         });
         __syncthreads();
         find_bin(sh, count, base, target);
@@ -431,21 +600,18 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
       }
       if (count) whole = above + in;
       /* the border's token, the only one left */
-      cut = prefix;
+      uint64_t token = prefix;
       if (shift) {
         __syncthreads();
-        each(lo64, hi64, [&](uint64_t c) {
+        each(bin, [&](float, uint64_t c) {
           if (c >> shift == prefix) sh.first = c;
         });
         __syncthreads();
-        cut = sh.first;
+        token = sh.first;
       }
+      cut = token;
       border = bin;
       __syncthreads();
-      if (count && row.by_p) { /* the histogram of what top-k keeps */
-        for (int i = tid; i < kFine; i += kT) sh.mass[i] = i < bin ? m0 : i == bin ? whole - ahead : 0;
-        __syncthreads();
-      }
     }
   }
   /* the kept mass of every part */
@@ -453,7 +619,11 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   if (wave < a.chunks) {
     if (row.by_k || row.by_p) {
       const int end = min(border, pass + 1);
-      for (int b = lane; b < end; b += GQ_WAVE) part += parts[wave].mass[b];
+      unsigned long long m[kBins / GQ_WAVE];
+#pragma unroll
+      for (int b = 0; b < kBins / GQ_WAVE; b++) m[b] = parts[wave].mass[b * GQ_WAVE + lane];
+#pragma unroll
+      for (int b = 0; b < kBins / GQ_WAVE; b++) part += b * GQ_WAVE + lane < end ? m[b] : 0;
       part = wave_sum(part);
     } else {
       part = parts[wave].kept;
@@ -462,10 +632,7 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   if (lane == 0 && wave < kChunks) sh.chunk[wave] = part;
   __syncthreads();
   if (border <= pass && border < kBins) {
-    const uint64_t hi64 = (uint64_t)(border ? lowest(border - 1) - 1 : key_of(row.top)) << 32 | 0xffffffffu;
-    each(cut, hi64, [&](uint64_t c) {
-      atomicAdd(&sh.chunk[(int)(~(uint32_t)c) / a.chunk], row.mass(value_of((uint32_t)(c >> 32))));
-    });
+    each(border, [&](float v, uint64_t c) { atomicAdd(&sh.chunk[(int)(~(uint32_t)c) / a.chunk], row.mass(v)); });
     __syncthreads();
   }
   unsigned long long whole = 0, before = 0;
@@ -485,16 +652,28 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   const int size = 256 * ((hi - lo + 256 * kT - 1) / (256 * kT));
   const auto kept = [&](float v, int i) -> unsigned long long {
     v = row.see(v);
-    return v > -INFINITY && comp_of(v, i) >= cut && (row.min_p == 0.f || row.passes(v)) ? row.mass(v) : 0ull;
+    const unsigned long long m = row.mass(v); /* 0 for what is never picked */
+    return comp_of(v, i) >= cut && row.passes(v) ? m : 0;
   };
-  for (int g = wave; g < kT; g += kW) {
-    const int from = lo + g * size;
-    unsigned long long s = 0;
-    if (from < hi) {
-      tokens<1>(x, from, min(hi, from + size), GQ_WAVE, lane, [&](float v, int i) { s += kept(v, i); });
-      s = wave_sum(s);
+  sh.mass[tid] = 0;
+  __syncthreads();
+  constexpr int G = 2; /* groups that a wave reads at once */
+  for (int g = wave; lo + g * size < hi; g += G * kW) {
+    unsigned long long s[G] = {};
+    for (int at = 4 * lane; at < size; at += 256) {
+      f32x4u v[G];
+#pragma unroll
+      for (int u = 0; u < G; u++) v[u] = four(x, lo + (g + u * kW) * size + at, hi);
+#pragma unroll
+      for (int u = 0; u < G; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[u] += kept(v[u][e], lo + (g + u * kW) * size + at + e);
     }
-    if (lane == 0) sh.mass[g] = s;
+#pragma unroll
+    for (int u = 0; u < G; u++) {
+      const unsigned long long t = wave_sum(s[u]);
+      if (lane == 0 && t) sh.mass[g + u * kW] = t;
+    }
   }
   if (tid == 0) sh.at = kT, sh.last = 0;
   __syncthreads();
@@ -502,7 +681,8 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   if (lane == 63) sh.wsum[wave] = sum;
   __syncthreads();
   unsigned long long at = before + sum;
-  for (int w = 0; w < wave; w++) at += sh.wsum[w];
+#pragma unroll
+  for (int w = 0; w < kW - 1; w++) at += w < wave ? sh.wsum[w] : 0;
   const uint64_t over = __ballot(own && (double)at > target), any = __ballot(own != 0);
   if (lane == 0) {
     if (over) atomicMin(&sh.at, tid + __builtin_ctzll(over));
@@ -516,12 +696,23 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   at = sh.before;
   const int from = lo + group * size, to = min(hi, from + size);
   int token = -1;
-  for (int b = from; b < to && (none || token < 0); b += GQ_WAVE) {
-    const int i = b + lane;
-    const unsigned long long m = i < to ? kept(x[i], i) : 0ull, c = wave_scan(m);
-    const uint64_t hit = __ballot(m && (none || (double)(at + c) > target));
-    if (hit) token = b + (none ? 63 - __builtin_clzll(hit) : __builtin_ctzll(hit));
-    at += __shfl(c, 63, 64);
+  for (int b = from; b < to && (none || token < 0); b += 256) {
+    const int i = b + 4 * lane;
+    const f32x4u v = four(x, i, to);
+    unsigned long long m[4], s = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) m[e] = kept(v[e], i + e), s += m[e];
+    const unsigned long long c = wave_scan(s);
+    unsigned long long run = at + c - s;
+    int mine = -1;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      run += m[e];
+      if (m[e] && (none || ((double)run > target && mine < 0))) mine = i + e;
+    }
+    const uint64_t hit = __ballot(mine >= 0);
+    if (hit) token = __builtin_amdgcn_readlane(mine, none ? 63 - __builtin_clzll(hit) : __builtin_ctzll(hit));
+    at += last_lane(c);
   }
   if (lane == 0) {
     a.tokens[r] = token;
@@ -556,12 +747,21 @@ extern "C" int gq_hip_sample_rows_dev(gq_ctx *c, const float *logits, int rows, 
   const int batch = std::min(rows, kRows);
   /* parts: enough workgroups for the chip, each with 4096 tokens or more */
   const int most = std::min(kChunks, (vocab + 4095) / 4096);
-  a.chunks = std::max(1, std::min(most, 512 / batch));
+  a.chunks = std::max(1, std::min(most, 1024 / batch));
   a.chunk = ((vocab + a.chunks - 1) / a.chunks + 3) / 4 * 4;
-  const size_t parts = sizeof(Part) * batch * a.chunks, tops = sizeof(uint64_t) * batch * a.n_tops;
-  char *ws = (char *)gq_ctx_paged_ws(c, parts + tops);
+  a.listers = std::max(1, std::min(a.chunks, 256 / batch));
+  const size_t lists = (size_t)batch * a.listers;
+  const size_t sizes[] = {sizeof(Part) * batch * a.chunks, sizeof(Border) * batch, sizeof(uint64_t) * batch * a.n_tops,
+                          sizeof(uint64_t) * kList * lists, sizeof(int) * lists};
+  size_t bytes = 0;
+  for (size_t n : sizes) bytes += n;
+  char *ws = (char *)gq_ctx_paged_ws(c, bytes);
   if (!ws) return gq_ctx_fail(c, -4, "sample_rows: workspace");
-  a.parts = (Part *)ws, a.tops = (uint64_t *)(ws + parts);
+  a.parts = (Part *)ws, ws += sizes[0];
+  a.borders = (Border *)ws, ws += sizes[1];
+  a.tops = (uint64_t *)ws, ws += sizes[2];
+  a.lists = (uint64_t *)ws, ws += sizes[3];
+  a.counts = (int *)ws;
   for (int r = 0; r < rows; r += batch) {
     const int n = std::min(batch, rows - r);
     a.x = logits + (long long)r * row_stride;
@@ -573,6 +773,7 @@ extern "C" int gq_hip_sample_rows_dev(gq_ctx *c, const float *logits, int rows, 
     a.logprobs = logprobs ? logprobs + r : nullptr;
     hipLaunchKernelGGL(tops_kernel, dim3(a.n_tops, n), dim3(kTopT), 0, ci.stream, a);
     hipLaunchKernelGGL(parts_kernel, dim3(a.chunks, n), dim3(kT), 0, ci.stream, a);
+    hipLaunchKernelGGL(list_kernel, dim3(a.listers, n), dim3(kT), 0, ci.stream, a);
     hipLaunchKernelGGL(draw_kernel, dim3(n), dim3(kT), 0, ci.stream, a);
   }
   return hipGetLastError() == hipSuccess ? 0 : gq_ctx_fail(c, -4, "sample_rows launch");
