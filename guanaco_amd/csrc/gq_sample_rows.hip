@@ -45,15 +45,15 @@ constexpr int kRows = 512;                     /* rows a launch: 40 MB of worksp
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 struct Part { /* what a part of a row leaves for the last launch */
-  unsigned long long mass[kBins];
-  uint32_t cnt[kBins];
+  unsigned long long mass[kBins]; /* of bins 0 .. this one */
+  uint32_t cnt[kBins];            /* tokens of them */
   unsigned long long kept; /* mass of what min_p keeps, for rows without top-k and top-p */
   int pass;                /* the last bin that min_p keeps */
   int pad;
 };
 
 struct Border { /* of a row, by the third launch */
-  unsigned long long mass[kBins]; /* of the whole row */
+  unsigned long long mass[kBins]; /* of bins 0 .. this one of the whole row */
   unsigned long long base, ahead; /* before the border's bin: the count (top-k) or mass, and the mass */
   int bin, from; /* bins from .. bin are listed */
   int pass;
@@ -158,7 +158,15 @@ __device__ __forceinline__ double fma_s(double a, double b, double c) {
   return d;
 }
 
-/* a row's parameters and what follows from them alone */
+/* a row's parameters: read before its largest logit is waited for */
+struct Params {
+  float T, p, min_p;
+  int k;
+  __device__ Params(const SampArgs &a, long long r)
+      : T(a.temperature ? a.temperature[r] : 1.f), p(a.top_p ? a.top_p[r] : 1.f), min_p(a.min_p ? a.min_p[r] : 0.f),
+        k(a.top_k ? a.top_k[r] : 0) {}
+};
+/* and what follows from them */
 struct Row {
   float top, T, min_p, scale;
   int k;
@@ -168,12 +176,8 @@ struct Row {
   double low; /* min_p keeps (v - top) c from here on */
   const double *tab;
 
-  __device__ Row(const SampArgs &a, long long r, uint64_t first, const double *t) : tab(t) {
-    T = a.temperature ? a.temperature[r] : 1.f;
-    k = a.top_k ? a.top_k[r] : 0;
-    p = a.top_p ? a.top_p[r] : 1.f;
-    min_p = a.min_p ? a.min_p[r] : 0.f;
-    min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
+  __device__ Row(const SampArgs &a, const Params &q, uint64_t first, const double *t) : T(q.T), k(q.k), p(q.p), tab(t) {
+    min_p = q.min_p > 0.f ? fminf(q.min_p, 1.f) : 0.f;
     if (p <= 0.f) k = 1, p = 1.f;
     by_k = k > 0 && k < a.vocab, by_p = p < 1.f;
     top = value_of((uint32_t)(first >> 32));
@@ -255,13 +259,16 @@ __global__ __launch_bounds__(kT, 8) void parts_kernel(SampArgs a) {
   __shared__ unsigned long long mass[kBins], kept;
   __shared__ uint32_t cnt[kBins];
   __shared__ int pass;
+  __shared__ unsigned long long wm[kBins / GQ_WAVE];
+  __shared__ uint32_t wc[kBins / GQ_WAVE];
   const int tid = threadIdx.x;
   const long long r = blockIdx.y;
   table(tab, a.S);
   for (int i = tid; i < kBins; i += kT) mass[i] = 0, cnt[i] = 0;
   if (tid == 0) kept = 0, pass = -1;
+  const Params q(a, r);
   const uint64_t f = first_of(a, r, &first);
-  const Row row(a, r, f, tab);
+  const Row row(a, q, f, tab);
   if (!f || !(row.T > 0.f)) return;
   const int lo = min(a.vocab, (int)blockIdx.x * a.chunk), hi = min(a.vocab, lo + a.chunk);
   const float *x = a.x + r * a.stride;
@@ -306,7 +313,18 @@ __global__ __launch_bounds__(kT, 8) void parts_kernel(SampArgs a) {
   else row.by_k ? fill(no, yes) : fill(no, no);
   if (last >= 0) atomicMax(&pass, last);
   __syncthreads();
-  for (int i = tid; i < kBins; i += kT) to.mass[i] = mass[i], to.cnt[i] = cnt[i];
+  unsigned long long m = 0, n = 0;
+  if (tid < kBins) {
+    m = wave_scan(mass[tid]), n = wave_scan(cnt[tid]);
+    if ((tid & 63) == 63) wm[tid >> 6] = m, wc[tid >> 6] = (uint32_t)n;
+  }
+  __syncthreads();
+  if (tid < kBins) {
+#pragma unroll
+    for (int w = 0; w < kBins / GQ_WAVE - 1; w++)
+      if (w < tid >> 6) m += wm[w], n += wc[w];
+    to.mass[tid] = m, to.cnt[tid] = (uint32_t)n;
+  }
   if (tid == 0) to.pass = pass;
 }
 
@@ -410,8 +428,9 @@ __global__ __launch_bounds__(kT) void list_kernel(SampArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long long r = blockIdx.y;
   const Part *parts = a.parts + r * a.chunks;
+  const Params q(a, r);
   const uint64_t first = first_of(a, r, &sh.first);
-  const Row row(a, r, first, sh.tab);
+  const Row row(a, q, first, sh.tab);
   if (!first || !(row.T > 0.f) || !(row.by_k || row.by_p)) return;
   /* the histogram of the whole row */
   unsigned long long m0 = 0;
@@ -430,19 +449,25 @@ __global__ __launch_bounds__(kT) void list_kernel(SampArgs a) {
 #pragma unroll
     for (int c = 0; c < kChunks; c++) c0 += c <= end ? m[c] : 0;
   }
-  static_assert(kT == 2 * kBins && kFine == 2 * kT, "a bin is two threads'");
-  if (tid < kBins) sh.mass[tid] = m0, sh.mass[tid + kBins] = 0;
-  else sh.cnt[tid - kBins] = c0, sh.cnt[tid] = 0;
-  sh.mass[tid + kT] = 0, sh.cnt[tid + kT] = 0;
+  static_assert(kT == 2 * kBins, "sums and counts are each half of the threads'");
+  if (tid < kBins) sh.mass[tid] = m0;
+  else sh.cnt[tid - kBins] = c0;
+  if (tid == 0) sh.at = kBins;
   __syncthreads();
-  const double target = row.by_k ? (double)row.k : (double)row.p * (double)block_sum(sh, m0);
-  find_bin(sh, row.by_k, 0, target);
-  const unsigned long long base = sh.before;
+  const double target = row.by_k ? (double)row.k : (double)row.p * (double)sh.mass[kBins - 1];
+  if (tid < kBins) {
+    const unsigned long long upto = row.by_k ? sh.cnt[tid] : sh.mass[tid];
+    const unsigned long long before = tid == 0 ? 0 : row.by_k ? sh.cnt[tid - 1] : sh.mass[tid - 1];
+    if ((double)upto >= target && (tid == 0 || !((double)before >= target))) sh.at = tid;
+  }
+  __syncthreads();
   /* a bin of mass 0: what is left weighs nothing.  With top-p to come, the
    * bins before top-k's border too, if they fit: top-p's is among them */
-  const int bin = sh.in ? sh.at : kBins;
-  const int from = bin < kBins && row.by_k && row.by_p && base + sh.n <= kList / 2 ? 0 : bin;
-  const unsigned long long ahead = block_sum(sh, tid < bin ? m0 : 0);
+  int bin = sh.at;
+  if (bin < kBins && sh.mass[bin] == (bin ? sh.mass[bin - 1] : 0)) bin = kBins;
+  const unsigned long long ahead = bin ? sh.mass[bin - 1] : 0;
+  const unsigned long long base = !row.by_k ? ahead : bin && bin < kBins ? sh.cnt[bin - 1] : 0;
+  const int from = bin < kBins && row.by_k && row.by_p && sh.cnt[bin] <= kList / 2 ? 0 : bin;
   Border &to = a.borders[r];
   if (blockIdx.x == 0) {
     if (tid < kBins) to.mass[tid] = m0;
@@ -478,8 +503,9 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   const float *x = a.x + r * a.stride;
   const Part *parts = a.parts + r * a.chunks;
   table(sh.tab, a.S);
+  const Params q(a, r);
   const uint64_t first = first_of(a, r, &sh.first);
-  const Row row(a, r, first, sh.tab);
+  const Row row(a, q, first, sh.tab);
   if (!first || !(row.T > 0.f)) { /* nothing to pick, or greedy */
     if (tid == 0) {
       a.tokens[r] = first ? (int)~(uint32_t)first : -1;
@@ -525,7 +551,8 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
   };
   if (row.by_k || row.by_p) {
     const Border &bd = a.borders[r];
-    const unsigned long long m0 = tid < kBins ? bd.mass[tid] : 0; /* bin t is thread t's */
+    const unsigned long long upto = tid < kBins ? bd.mass[tid] : 0; /* of bins 0 .. tid */
+    unsigned long long whole = bd.mass[kBins - 1];                  /* mass of what top-k keeps */
     if (row.min_p > 0.f) pass = bd.pass;
     { /* the third launch's lists, one behind the other */
       const int m = lane < a.listers ? a.counts[r * a.listers + lane] : 0;
@@ -539,28 +566,29 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
       const int all = __builtin_amdgcn_readlane(sum, kChunks - 1);
       listed = listed && all <= kList;
       if (listed) {
-        for (int l = 0; l < a.listers; l++) {
-          const int from = l ? __builtin_amdgcn_readlane(sum, l - 1) : 0, k = __builtin_amdgcn_readlane(m, l);
-          for (int j = tid; j < k; j += kT) sh.list[from + j] = a.lists[(r * a.listers + l) * kList + j];
-        }
+        const int l = wave % a.listers, by = kW / a.listers, k = __builtin_amdgcn_readlane(m, l);
+        const int from = l ? __builtin_amdgcn_readlane(sum, l - 1) : 0;
+        if (wave / a.listers < by)
+          for (int j = wave / a.listers * GQ_WAVE + lane; j < k; j += by * GQ_WAVE)
+            sh.list[from + j] = a.lists[(r * a.listers + l) * kList + j];
         const int share = (all + kW - 1) / kW, at = min(all, wave * share);
         list = sh.list + at, n = min(all - at, share);
         b0 = bd.from, b1 = bd.bin;
       }
       __syncthreads();
     }
-    unsigned long long whole = 0; /* mass of what top-k keeps */
-    if (!row.by_k) whole = block_sum(sh, m0);
     for (int by = row.by_k ? 0 : 1; by < (row.by_p ? 2 : 1); by++) {
       const bool count = by == 0;
       const double target = count ? (double)row.k : (double)row.p * (double)whole;
       int bin = bd.bin;
       unsigned long long base = bd.base; /* count or mass before the border's bin */
       if (!count && row.by_k) { /* the histogram of what top-k keeps */
-        for (int i = tid; i < kFine; i += kT) sh.mass[i] = i < border ? m0 : i == border ? whole - bd.ahead : 0;
+        if (tid < kBins) sh.mass[tid] = tid < border ? upto : whole;
+        if (tid == 0) sh.at = kBins - 1;
         __syncthreads();
-        find_bin(sh, false, 0, target);
-        bin = sh.at, base = sh.before;
+        if (tid < kBins && (double)sh.mass[tid] >= target && (tid == 0 || !((double)sh.mass[tid - 1] >= target))) sh.at = tid;
+        __syncthreads();
+        bin = sh.at, base = bin ? sh.mass[bin - 1] : 0;
       }
       unsigned long long above = bd.ahead, in = 0; /* mass before it; of the border itself */
       if (count && bin == kBins) { /* what is left weighs nothing */
@@ -615,21 +643,10 @@ __global__ __launch_bounds__(kT) void draw_kernel(SampArgs a) {
     }
   }
   /* the kept mass of every part */
-  unsigned long long part = 0;
-  if (wave < a.chunks) {
-    if (row.by_k || row.by_p) {
-      const int end = min(border, pass + 1);
-      unsigned long long m[kBins / GQ_WAVE];
-#pragma unroll
-      for (int b = 0; b < kBins / GQ_WAVE; b++) m[b] = parts[wave].mass[b * GQ_WAVE + lane];
-#pragma unroll
-      for (int b = 0; b < kBins / GQ_WAVE; b++) part += b * GQ_WAVE + lane < end ? m[b] : 0;
-      part = wave_sum(part);
-    } else {
-      part = parts[wave].kept;
-    }
+  if (tid < a.chunks) {
+    const int end = min(border, pass + 1);
+    sh.chunk[tid] = !(row.by_k || row.by_p) ? parts[tid].kept : end ? parts[tid].mass[end - 1] : 0;
   }
-  if (lane == 0 && wave < kChunks) sh.chunk[wave] = part;
   __syncthreads();
   if (border <= pass && border < kBins) {
     each(border, [&](float v, uint64_t c) { atomicAdd(&sh.chunk[(int)(~(uint32_t)c) / a.chunk], row.mass(v)); });
