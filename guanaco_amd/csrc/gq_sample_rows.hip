@@ -18,10 +18,18 @@
  * atomics may add them, the same call gives the same token, and neither
  * depends on how many workgroups share a row.
  *
- * Three launches: the largest logit of every 4096 tokens; the histograms of
- * `chunks` parts of each row; one workgroup a row for the borders and the draw,
- * which reads the row once more for the border's bin (tokens between two
- * logits: a compare each) and one part of it for the draw.
+ * Four launches: the largest logit of every 4096 tokens; the histograms of a
+ * row's parts; the border of top-k (or else top-p) and a list of the tokens in
+ * its bin; one workgroup a row for the rest, which reads one part of it again
+ * for the draw.  The middle two are shared by as many workgroups as fill the
+ * chip, since one alone reads a row of 128256 in 10 us.
+ *
+ * At 128256 tokens (kernel times): 128 rows with filters of their own 11 us for
+ * the largest logits (65.7 MB at 5.8 TB/s, what a copy reaches), 27 for the
+ * histograms (bound by the 64-bit LDS atomics, one a token: 60 cycles a wave
+ * of them; with half the vector instructions it took 25 instead of 27), 18 for
+ * the lists (65.7 MB again) and 24 for the rest, 80 us together; one row 4, 7, 9 and 19
+ * us, bound by the memory latencies and barriers one after the other.
  */
 #include <algorithm>
 #include <cmath>
@@ -424,13 +432,18 @@ __device__ __forceinline__ int list_tokens(const Row &row, const float *x, int l
 /* a row's border of top-k, or else of top-p: its bin, and the tokens of it
  * among the parts that a workgroup looks through */
 __global__ __launch_bounds__(kT) void list_kernel(SampArgs a) {
-  __shared__ Shared sh;
+  __shared__ struct {
+    unsigned long long mass[kBins];
+    uint32_t cnt[kBins];
+    uint64_t list[kList], first;
+    int at, n[kW];
+  } sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const long long r = blockIdx.y;
   const Part *parts = a.parts + r * a.chunks;
   const Params q(a, r);
   const uint64_t first = first_of(a, r, &sh.first);
-  const Row row(a, q, first, sh.tab);
+  const Row row(a, q, first, nullptr);
   if (!first || !(row.T > 0.f) || !(row.by_k || row.by_p)) return;
   /* the histogram of the whole row */
   unsigned long long m0 = 0;
@@ -481,13 +494,13 @@ __global__ __launch_bounds__(kT) void list_kernel(SampArgs a) {
   const int per = (a.chunks + a.listers - 1) / a.listers * a.chunk;
   const int lo = min(a.vocab, (int)blockIdx.x * per), hi = min(a.vocab, lo + per);
   if (bin < kBins) n = list_tokens<8>(row, a.x + r * a.stride, lo, hi, from, bin, sh.list + wave * kShare);
-  if (lane == 0) sh.wsum[wave] = n;
+  if (lane == 0) sh.n[wave] = n;
   __syncthreads();
   int at = 0, all = 0;
   bool fits = true;
 #pragma unroll
   for (int w = 0; w < kW; w++) {
-    const int m = (int)sh.wsum[w];
+    const int m = sh.n[w];
     at += w < wave ? m : 0, all += m, fits = fits && m <= kShare;
   }
   const long long l = r * a.listers + blockIdx.x;

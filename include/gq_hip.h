@@ -503,7 +503,8 @@ int gq_hip_paged_prompt_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *
  * to tokens[rows], and log(w / whole sum) to logprobs[rows] (may be NULL; 0
  * for temperature 0).  The weights and sums are exact to 2^-45 of the largest
  * and the same in every call.  NaN and -infinity are never picked; a row of
- * nothing else gets -1 and -infinity.  Asynchronous on the context's stream.
+ * nothing else gets -1 and -infinity.  Asynchronous on the context's stream;
+ * workspace is the context's.
  * gq_hip_sample_dev follows the reference's samplers for one row instead:
  * another order of the sums, one of the filters, and libc's rand(). */
 int gq_hip_sample_rows_dev(gq_ctx *ctx, const float *logits, int rows, int vocab, int row_stride,

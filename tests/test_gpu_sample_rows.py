@@ -184,3 +184,40 @@ def test_repeated_calls_give_the_same(ctx):
     for _ in range(3):
         b = run(ctx, x, 1.0, 0, 0.97, 0.0, u)
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("rows", [1, 3, 70, 300, 600])
+def test_rows_shared_by_workgroups(ctx, rows):
+    """From one row to more than a launch takes: 16 parts a row to one, lists
+    that hold all before top-k's border, lists that do not fit, none."""
+    V = 66000 if rows < 100 else 9001
+    r = np.random.default_rng(rows)
+    f = [(3000, 0.9, 0.0), (6000, 0.9, 0.0), (6000, 0.999, 0.001), (8990, 0.5, 0.2), (50, 1.0, 0.0), (0, 0.97, 0.0), (0, 1.0, 0.0), (V, 0.3, 0.01)]
+    k, p, m = (np.array(v) for v in zip(*[f[(i + rows) % len(f)] for i in range(rows)]))
+    x = logits(rows, V, rows + 20)
+    check(ctx, x, r.choice([0.6, 1.0, 1.7], rows).astype(np.float32), k.astype(np.int32), p.astype(np.float32), m.astype(np.float32),
+          r.random(rows, np.float32), stride=V + 3)
+
+
+@pytest.mark.parametrize("at", [0, 3, 30000])
+def test_border_tokens_side_by_side(ctx, at):
+    """9000 neighbours share the border's bin: more than fit a list, and all of
+    them those of few waves; and 700, more than one wave's share of it."""
+    for n in (700, 9000):
+        x = logits(4, 128256, n + at) - 20
+        x[:, at:at + n] = 3 + 1e-4 * np.random.default_rng(n).random((4, n))
+        x[:, at + n + 5] = 4
+        x = x.astype(np.float32)
+        u = np.array([0.01, 0.3, 0.6, 0.99], np.float32)
+        for k, p, m in [(n // 2, 1.0, 0.0), (0, 0.7, 0.0), (n - 50, 0.6, 0.2), (n // 2, 0.9, 0.9)]:
+            check(ctx, x, 1.0, k, p, m, u)
+
+
+def test_one_call_of_many_rows_is_many_calls(ctx):
+    """A row's token does not depend on how many workgroups share its row."""
+    x = logits(33, 50257, 9)
+    u = np.random.default_rng(10).random(33, np.float32)
+    a = run(ctx, x, 0.9, 400, 0.93, 0.001, u)
+    for i in (0, 7, 32):
+        b = run(ctx, x[i:i + 1], 0.9, 400, 0.93, 0.001, u[i:i + 1])
+        assert a[0][i] == b[0][0] and a[1][i] == b[1][0]
