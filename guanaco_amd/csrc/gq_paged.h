@@ -39,6 +39,11 @@ __device__ __forceinline__ int pgd_seq_of(const PgdBatch &b, int t) {
   return b.n_seqs;
 }
 
+/* Positions before the call's tokens.  None from max_len on exists, so that a
+ * larger number says no more than max_len; the sum with a token's number then
+ * stays within 31 bits (max_len and n_tokens are 2^30 at most). */
+__device__ __forceinline__ int pgd_before(const PgdBatch &b, int pos) { return min(pos, b.max_len); }
+
 /* (row of the first new token, their number) of a sequence, s uniform in the
  * wave; none where the rows are not in the packed arrays */
 __device__ __forceinline__ int2 pgd_rows(const PgdBatch &b, int s) {

@@ -81,9 +81,9 @@ __device__ __forceinline__ bool find_rows(const PgdPages &c, const PgdBatch &b, 
     }
     const bool in = t < b.n_tokens && s < b.n_seqs;
     const int sc = in ? s : 0;
-    const int r0 = b.first ? gld<int>(b.first + sc) : t, p0 = gld<int>(b.pos + sc);
-    o.t[u] = in && t >= r0 ? t : -1;
-    o.p[u] = p0 < 0 ? -1 : p0 + (t - r0);
+    const int r0 = b.first ? gld<int>(b.first + sc) : t, p0 = pgd_before(b, gld<int>(b.pos + sc));
+    o.t[u] = in && r0 >= 0 && t >= r0 ? t : -1;
+    o.p[u] = o.t[u] < 0 || p0 < 0 ? -1 : p0 + (t - r0);
     o.page[u] = o.t[u] < 0 || o.p[u] < 0 ? -1 : pgd_page(c, b, sc, o.p[u]);
   }
   return true;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
 __device__ __forceinline__ bool decode_row(const AttArgs &a, int s, int &row, int &len) {
   const int2 rn = pgd_rows(a.b, s);
   if (rn.y < 1) return false;
-  const int p0 = gq_sld<int>(a.b.pos + s);
+  const int p0 = pgd_before(a.b, gq_sld<int>(a.b.pos + s));
   row = rn.x + rn.y - 1;
   len = p0 < 0 ? 0 : min(p0 + rn.y, a.b.max_len);
   return true;
@@ -612,7 +612,7 @@ int check_cache(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype) {
     return gq_ctx_fail(c, -1, "paged: page_size is a power of two from 16 to 1024");
   if (b->n_seqs < 0 || b->n_tokens < 0) return gq_ctx_fail(c, -1, "paged: negative size of the batch");
   if (b->n_seqs && (!b->table || !b->pos || b->table_stride < 1 || b->max_len < 0)) return gq_ctx_fail(c, -1, "paged: incomplete batch");
-  if (b->max_len > (1 << 30)) return gq_ctx_fail(c, -1, "paged: max_len passes 2^30");
+  if (b->max_len > (1 << 30) || b->n_tokens > (1 << 30)) return gq_ctx_fail(c, -1, "paged: max_len or n_tokens passes 2^30");
   if (!b->first && b->n_tokens < b->n_seqs) return gq_ctx_fail(c, -1, "paged: fewer rows than sequences");
   if (b->n_seqs && (long long)b->max_len > (long long)b->table_stride * p->page_size)
     return gq_ctx_fail(c, -5, "paged: max_len passes the page table");

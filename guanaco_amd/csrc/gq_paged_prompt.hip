@@ -27,7 +27,7 @@ __device__ __forceinline__ Tile find_tile(const PgdBatch &b, int tpt, int id) {
     const int q = s0 + lane, qc = min(q, b.n_seqs - 1), cnt = min(GQ_WAVE, b.n_seqs - s0);
     int r0 = qc, r1 = qc + 1;
     if (b.first) r0 = gld<int>(b.first + qc), r1 = gld<int>(b.first + qc + 1);
-    int p0 = gld<int>(b.pos + qc);
+    int p0 = pgd_before(b, gld<int>(b.pos + qc));
     const bool in = q < b.n_seqs && r0 >= 0 && r1 <= b.n_tokens && r1 > r0;
     if (!in) r0 = r1 = 0;
     int sq = q;
@@ -661,7 +661,7 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(AttArgs a, int tpt) {
   if (s >= a.b.n_seqs) return;
   const int2 rn = pgd_rows(a.b, s);
   if (row < rn.x || row >= rn.x + rn.y) return;
-  const int parts = tile_blocks(a, gq_sld<int>(a.b.pos + s), min((row - rn.x) / tpt * tpt + tpt, rn.y) - 1).y;
+  const int parts = tile_blocks(a, pgd_before(a.b, gq_sld<int>(a.b.pos + s)), min((row - rn.x) / tpt * tpt + tpt, rn.y) - 1).y;
   if (parts <= 1) return; /* its one part has written the result */
   for (int i = threadIdx.x; i < a.n_heads * (HD / 4); i += 256) {
     const int qh = i / (HD / 4), dim = 4 * (i % (HD / 4));

@@ -440,7 +440,8 @@ typedef struct {
  * new token in the packed arrays of n_tokens rows, first[s + 1] - first[s]
  * their number (0 is allowed).  first NULL: one token each, row s.  max_len: no
  * sequence is longer, its new tokens included; positions from there on do not
- * exist either.  It sizes launches and workspaces, so a close bound is faster. */
+ * exist either.  It sizes launches and workspaces, so a close bound is faster.
+ * max_len and n_tokens: 2^30 at most. */
 typedef struct {
   const int32_t *table, *pos, *first;
   int n_seqs, table_stride, n_tokens, max_len;

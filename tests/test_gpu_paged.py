@@ -352,3 +352,28 @@ def test_empty_batches(ctx):
     w.batch.n_seqs = 0
     assert (attend(ctx, w, 4, F32, "paged_decode_dev")[1] == 5).all()
     w.free()
+
+
+@pytest.mark.parametrize("pos", [2 ** 31 - 1, 2 ** 31 - 3, 1 << 30])
+@pytest.mark.parametrize("cache", [F32, BF16, I8])
+def test_positions_near_the_end_of_int32(ctx, cache, pos):
+    """Device positions whose sum with a token's number passes 31 bits: past
+    max_len all the same."""
+    w = World(18, [93, 40], [7, 3], 2, 64, cache, 16)
+    w.hist[0] = pos
+    w.upload(ctx, H)
+    w.at = [(0, 99)] * 7 + [(1, 40 + i) for i in range(3)]
+    for entry, rows in (("paged_decode_dev", [6, 9]), ("paged_prompt_dev", range(10))):
+        q, got = attend(ctx, w, 4, F32, entry)
+        check_attention(w, q, got, rows, F32, entry == "paged_prompt_dev")
+    x = ctx.upload(np.ones((10, 128), np.float32))
+    before = w.download(0)[0]
+    ctx.paged_append_dev(w.pages, w.batch, F32, 0, None, 0, None, 0, x, 128, x, 128, None, 0)
+    after = w.download(0)[0]
+    for i in range(3):
+        g, o = w.slot(1, 40 + i)
+        after[g, :, o] = before[g, :, o]
+    assert after.tobytes() == before.tobytes()
+    ctx.paged_read_dev(w.pages, w.batch, F32, x, 128, x, 128)
+    assert (x.download().reshape(10, 128)[:7] == 0).all()
+    w.free()

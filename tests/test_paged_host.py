@@ -108,7 +108,7 @@ def test_taken_and_run_on_the_contexts_device(lib, call):
     (dict(p=pages(page_size=0)), -1), (dict(p=pages(page_size=-64)), -1),
     (dict(b=batch(table=None)), -1), (dict(b=batch(pos=None)), -1), (dict(b=batch(n_seqs=-1)), -1),
     (dict(b=batch(n_tokens=-1)), -1), (dict(b=batch(table_stride=0)), -1), (dict(b=batch(max_len=-1)), -1),
-    (dict(b=batch(first=None, n_tokens=3)), -1), (dict(b=batch(max_len=(1 << 30) + 1, table_stride=1 << 25)), -1), (dict(b=batch(max_len=641)), -5),
+    (dict(b=batch(first=None, n_tokens=3)), -1), (dict(b=batch(max_len=(1 << 30) + 1, table_stride=1 << 25)), -1), (dict(b=batch(max_len=641)), -5), (dict(b=batch(n_tokens=(1 << 30) + 1)), -1),
 ])
 def test_refused_by_every_entry(lib, call, what, rc):
     lib.fake_reset(0)
