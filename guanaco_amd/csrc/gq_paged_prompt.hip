@@ -112,7 +112,9 @@ __device__ __forceinline__ void pin(gq_bf16x8 &v, float &f) {
  * and for int8 without 64 products by scales a lane and block (2.5 -> 1.8 us).
  *
  * Keys that do not exist are masked, and their V zeros in LDS, so that what stale
- * memory holds cannot reach a sum.
+ * memory holds cannot reach a sum.  So are infinities and NaN of V in the blocks that
+ * only some rows see whole (a masked probability of 0 times them is no 0): those
+ * that see them get them at the end.  The check costs 1 to 3%.
  *
  * The blocks of a tile come in parts of at most a.chunk, a workgroup each, where
  * the tiles alone would leave CUs idle; prompt_merge_kernel joins them. */
@@ -139,7 +141,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   constexpr int VTH = 16 * HD / 4;           /* threads with four keys x four dims of V */
   constexpr int NQ = NX == 3 ? 2 : 1;        /* planes of Q in registers; the third in LDS */
   constexpr int QLO = NB * 2 * NK * KPL, SCL = QLO + (NX == 3 ? RG * NSL * 1024 : 0);
-  constexpr int LDS = std::max(SCL + (CODES ? (4 + NB) * kKeys * 4 : 0), /* scales: four blocks of K's, NB of V's */
+  constexpr int ODD = SCL + (CODES ? (4 + NB) * kKeys * 4 : 0);          /* scales: four blocks of K's, NB of V's */
+  constexpr int LDS = std::max(ODD + 32, /* a flag per wave */
                                KH == 2 ? RG * 64 * 4 * (ND * 16 + 2) : 0);          /* the halves' exchange */
   __shared__ __attribute__((aligned(16))) uint8_t smem_[LDS];
   GQ_LDS uint8_t *smem = (GQ_LDS uint8_t *)smem_;
@@ -259,8 +262,14 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       }
     }
   };
+  /* blocks that not all of the tile's rows see whole */
+  const int pmin = sees(0);
+  uint32_t odd = 0; /* this wave has zeroed some */
+  auto partial = [&](int b) { return b * kKeys + kKeys - 1 > pmin; };
   /* the loaded K or V of block b into buffer buf; V's rows that do not exist are
-   * zeros (K's scores are masked) */
+   * zeros (K's scores are masked), and so are in a partial block the values that
+   * are no numbers: times a masked probability they would reach rows that do not
+   * see them.  Those that do get them at the end. */
   auto stagek = [&](int b, int buf, uint32_t (&kr)[KI][KW], float sc) {
     const uint32_t kb = (uint32_t)(buf * 2 * NK * KPL);
 #pragma unroll
@@ -302,6 +311,35 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         const bool there = (ok >> (va >> 2 & 3) & 1) && b * kKeys + 4 * va + i <= pmax;
 #pragma unroll
         for (int e = 0; e < VW; e++) vr[i][e] = there ? vr[i][e] : 0u;
+      }
+    }
+    if (partial(b)) {
+      /* added to an exponent of ones, one in its last place carries; fp32 values
+       * that are to be bf16: from those on that round to an infinity */
+      constexpr uint32_t ex = CT == GQ_BF16 ? 0x7f807f80u : 0x7fffffffu, top = CT == GQ_BF16 ? 0x80008000u : 0x80000000u;
+      constexpr uint32_t one = CT == GQ_BF16 ? 0x00800080u : CT == GQ_F32 && NK == 1 ? 0x00808000u : 0x00800000u;
+      uint32_t bad = 0;
+      if constexpr (CODES) {
+        bad = wv == 1 ? (__builtin_bit_cast(uint32_t, sc) & ex) + one : 0u;
+      } else if (vtask) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int e = VALUES ? 1 : 0; e < VW; e++) bad |= (vr[i][e] & ex) + one;
+      }
+      if (__ballot((bad & top) != 0)) {
+        odd = 1;
+        if constexpr (CODES) {
+          sc = bad & top ? 0.f : sc;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = VALUES ? 1 : 0; e < VW; e++) {
+              const uint32_t c = ((vr[i][e] & ex) + one) & top;
+              vr[i][e] &= ~(CT == GQ_BF16 ? (c >> 15) * 0xffffu : c ? ~0u : 0u);
+            }
+        }
       }
     }
     if (vtask) {
@@ -607,6 +645,32 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         __syncthreads();
       }
     }
+  }
+  /* The values of partial blocks that are no numbers, to the outputs of the rows
+   * that see them: times a weight above zero an infinity or NaN is the same. */
+  if (lane == 0) lst<uint32_t>(smem, ODD + 4 * wv, odd);
+  __syncthreads();
+  {
+    const uint4 f = lld<uint4>(smem, ODD), f1 = lld<uint4>(smem, ODD + 16);
+    odd = (uint32_t)__builtin_amdgcn_readfirstlane((int)(f.x | f.y | f.z | f.w | f1.x | f1.y | f1.z | f1.w));
+  }
+  for (int u = b0 * kKeys; odd && u < min(b1 * kKeys, pmax + 1); u++) {
+    const int page = partial(u / kKeys) && (KH == 1 || (u >> 5 & 1) == kh) ? pgd_page_u(a.c, a.b, s, u) : -1;
+    if (page < 0) continue;
+    const size_t at = pgd_row(a.c, page, g, u & ps);
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const size_t i = at * HD + 32 * d + 8 * (e >> 2) + 4 * h + (e & 3);
+        float x;
+        if constexpr (CT == GQ_F32) x = gld<float>((const float *)a.c.v + i);
+        else if constexpr (CT == GQ_BF16) x = pgd_lo(gld<uint16_t>((const uint16_t *)a.c.v + i));
+        else x = (float)*(const GQ_GLOBAL int8_t *)(a.c.v + i) * gld<float>(a.c.vs + at);
+        if constexpr (NX == 1) x = pgd_lo(pgd_pack(x, x));
+        if (u <= cpos && (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) == 0x7f800000u) o[d][e] += x;
+        __builtin_amdgcn_sched_barrier(0); /* one load at a time: no registers beside the outputs */
+      }
   }
   l += __shfl_xor(l, 32, 64);
   if constexpr (KH == 2) { /* kh = 1 hands (m, l, O) to kh = 0 */

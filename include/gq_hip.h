@@ -483,7 +483,8 @@ int gq_hip_paged_decode_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *
  * sequence s over positions 0 .. pos[s] + t, whose rows are in the cache.
  * GQ_F32 queries keep fp32 accuracy throughout; with GQ_BF16 ones the
  * probabilities are rounded to bf16 before they meet V, and the values of a
- * GQ_F32 or GQ_I8_ROWS cache before they meet either. */
+ * GQ_F32 or GQ_I8_ROWS cache before they meet either.  An infinity or NaN in
+ * the cache reaches the tokens that see its position and no others. */
 int gq_hip_paged_prompt_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
                             const void *q, int q_stride, void *out, int out_stride);
 

@@ -377,3 +377,43 @@ def test_positions_near_the_end_of_int32(ctx, cache, pos):
     ctx.paged_read_dev(w.pages, w.batch, F32, x, 128, x, 128)
     assert (x.download().reshape(10, 128)[:7] == 0).all()
     w.free()
+
+
+ODD = [float("nan"), float("inf"), -float("inf")]
+
+
+@pytest.mark.parametrize("xt", [F32, BF16])
+@pytest.mark.parametrize("cache", [F32, BF16, I8])
+@pytest.mark.parametrize("case", [(8, 2, 64, 16, [5, 0], [90, 40]), (16, 8, 128, 64, [70, 1], [150, 3]), (12, 1, 128, 32, [0, 300], [33, 130]),
+                                  (4, 4, 64, 128, [1000, 0], [300, 64])])
+def test_values_that_are_no_numbers_stay_in_their_future(ctx, case, cache, xt):
+    """K and V rows with an infinity or NaN at one of a prompt's own positions:
+    the tokens before it are as if they were not there, bit for bit, those from
+    it on are no numbers in V's dimensions (in all of them for K's and for a row
+    of int8 codes, whose scale is NaN then)."""
+    nh, nkv, hd, page, hist, new = case
+    clean = World(21, hist, new, nkv, hd, cache, page, pad=1).upload(ctx, H)
+    q, ref = attend(ctx, clean, nh, xt, "paged_prompt_dev")
+    clean.free()
+    for which in (0, 1):
+        for n, t in enumerate([0, 1, new[0] // 2, new[0] - 1]):
+            w = World(21, hist, new, nkv, hd, cache, page, pad=1)
+            g, o = w.slot(0, hist[0] + t)
+            head, dim, v = n % nkv, (37 * n + 5) % hd, np.float32(ODD[n % 3])
+            if cache == I8:
+                w.pools[which][1][g, head, o] = np.nan
+            else:
+                w.pools[which][0][g, head, o, dim] = enc(v, cache)
+            w.upload(ctx, H)
+            got = attend(ctx, w, nh, xt, "paged_prompt_dev")[1]
+            w.free()
+            a, b = dec(got, xt).reshape(-1, nh, hd), dec(ref, xt).reshape(-1, nh, hd)
+            G = nh // nkv
+            hit = np.zeros(a.shape, bool)
+            if cache == I8:
+                hit[t:new[0], head * G:(head + 1) * G] = True
+            else:
+                hit[t:new[0], head * G:(head + 1) * G, dim if which else slice(None)] = True
+            assert np.array_equal(a[~hit], b[~hit]), (which, t)
+            if which or cache == I8 or np.isnan(v):  # an infinite score may also weigh nothing
+                assert not np.isfinite(a[hit]).any(), (which, t)
