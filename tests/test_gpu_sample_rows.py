@@ -12,6 +12,8 @@ logprobs: the float32 rounding of a float64 value, 2^-24 relative, and 1e-12."""
 import numpy as np
 import pytest
 
+import guanaco_amd.hip as H
+
 pytestmark = pytest.mark.gpu
 
 
@@ -221,3 +223,53 @@ def test_one_call_of_many_rows_is_many_calls(ctx):
     for i in (0, 7, 32):
         b = run(ctx, x[i:i + 1], 0.9, 400, 0.93, 0.001, u[i:i + 1])
         assert a[0][i] == b[0][0] and a[1][i] == b[1][0]
+
+
+@pytest.mark.parametrize("T", [np.inf, 3e38, 1e-42, 1e-37])
+def test_temperatures_at_the_ends(ctx, T):
+    x = logits(4, 5000, 12)
+    x[1] *= 1e37
+    x[2, :3] = 3.4e38
+    x[3] *= 1e-38
+    u = np.array([0.13, 0.5, 0.77, 0.91], np.float32)
+    for k, p, m in [(0, 1.0, 0.0), (33, 1.0, 0.0), (0, 0.7, 0.0), (2500, 0.51, 0.3)]:
+        check(ctx, x, np.float32(T), k, p, m, u, exact=True)
+
+
+def test_the_largest_vocabulary(ctx):
+    """2^20 tokens, a stride of their number and one: rows that start 4-byte
+    aligned, borders in bins of more tokens than a list holds."""
+    x = logits(3, 1 << 20, 13)
+    u = np.array([0.2, 0.55, 0.9], np.float32)
+    for T, k, p, m in [(1.0, 0, 0.9, 0.0), (3.0, 100000, 0.95, 0.01), (20.0, 0, 0.5, 0.0), (1.0, 50, 0.9, 0.0)]:
+        check(ctx, x, np.float32(T), k, p, m, u, stride=(1 << 20) + 1)
+
+
+def test_many_rows_of_the_largest_vocabulary(ctx):
+    """Parts of more than 2^18 tokens, which are drawn from in larger groups;
+    offsets past 2^28 elements."""
+    rows, V = 300, 1 << 20
+    x, on = logits(3, V, 14), [0, 151, 299]
+    b = ctx.alloc(4 * rows * V)
+    small = ctx.upload(np.zeros(V, np.float32))
+    for i in range(rows):
+        src = ctx.upload(x[on.index(i)]) if i in on else small
+        assert H.lib.gq_hip_copy_dev(ctx.h, b.ptr + 4 * V * i, src.ptr, 4 * V) == 0
+        ctx.sync()
+        if i in on:
+            src.free()
+    u = np.random.default_rng(15).random(rows, np.float32)
+    ub, tok = ctx.upload(u), ctx.upload(np.full(rows, -7, np.int32))
+    f = lambda v, t: ctx.upload(np.full(rows, v, t))  # noqa: E731
+    k, p, m = f(70000, np.int32), f(0.8, np.float32), f(0.001, np.float32)
+    for with_filters in (False, True):
+        ctx.sample_rows_dev(b, rows, V, V, None, k if with_filters else None, p if with_filters else None, m if with_filters else None, ub, tok)
+        got = tok.download(np.int32)
+        for j, i in enumerate(on):
+            t, _, far = reference(x[j], np.float32(1), 70000 if with_filters else 0, 0.8 if with_filters else 1.0, 0.001 if with_filters else 0.0, u[i])
+            assert far > V * 2.0 ** -44 and got[i] == t, (i, got[i], t, far)
+        n = int(np.ceil(np.float64(np.float32(0.8)) * 70000)) if with_filters else V  # equal logits: the first n
+        for i in (1, 150, 298):
+            assert got[i] == int(np.float64(u[i]) * n)
+    for v in (b, small, ub, tok, k, p, m):
+        v.free()
