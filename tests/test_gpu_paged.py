@@ -417,3 +417,38 @@ def test_values_that_are_no_numbers_stay_in_their_future(ctx, case, cache, xt):
             assert np.array_equal(a[~hit], b[~hit]), (which, t)
             if which or cache == I8 or np.isnan(v):  # an infinite score may also weigh nothing
                 assert not np.isfinite(a[hit]).any(), (which, t)
+
+
+def some_rows(w, n=40, seed=30):
+    """the first and last token of a few sequences, and others"""
+    r = np.random.default_rng(seed)
+    ends = [t for s in r.permutation(len(w.new))[:8] if w.new[s] for t in (w.first[s], w.first[s + 1] - 1)]
+    return sorted({*ends, *r.integers(0, len(w.at), n)})
+
+
+@pytest.mark.parametrize("xt", [F32, BF16])
+@pytest.mark.parametrize("cache", [F32, BF16, I8])
+def test_prompts_of_many_sequences(ctx, cache, xt):
+    """150 sequences, more than a wave looks through at once, longest first."""
+    r = np.random.default_rng(31)
+    hist, new = r.integers(-1, 200, 150), r.integers(0, 40, 150)
+    w = World(32, hist.tolist(), new.tolist(), 2, 64, cache, 16, pad=5).upload(ctx, H)
+    q, got = attend(ctx, w, 8, xt, "paged_prompt_dev")
+    check_attention(w, q, dec(got, xt), some_rows(w), xt, True)
+    idle = [t for t, (s, p) in enumerate(w.at) if p < 0]
+    assert idle and not dec(got[idle], xt).any() and (got[len(w.at):] == 5).all()
+    w.free()
+
+
+@pytest.mark.parametrize("xt", [F32, BF16])
+@pytest.mark.parametrize("cache", [F32, BF16, I8])
+@pytest.mark.parametrize("hist,new", [([9000], [1]), ([7001, 30, 0], [5, 130, 1]), ([500], [2000]), ([0, 0, 100], [1500, 1, 999])])
+def test_prompts_in_parts_and_in_large_tiles(ctx, hist, new, cache, xt):
+    """Few tokens over many keys, whose parts are joined, beside sequences of
+    fewer parts; and enough of them for the larger tiles."""
+    w = World(33, hist, new, 4, 128, cache, 64, pad=2).upload(ctx, H)
+    q, got = attend(ctx, w, 16, xt, "paged_prompt_dev")
+    check_attention(w, q, dec(got, xt), some_rows(w, 12), xt, True)
+    again = attend(ctx, w, 16, xt, "paged_prompt_dev")[1]
+    assert np.array_equal(got, again) and (got[len(w.at):] == 5).all()
+    w.free()

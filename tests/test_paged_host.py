@@ -180,3 +180,28 @@ def test_sampling_refused(lib, what):
 def test_sampling_of_no_rows(lib):
     lib.fake_reset(0)
     assert sample(lib, rows=0, logits=None) == 0 and lib.fake_launches() == 0
+
+
+def test_workspace_refused(lib):
+    """A call that needs workspace and gets none: -4, nothing launched."""
+    long = dict(p=pages(page_size=128, n_pages=4000), b=batch(n_seqs=1, n_tokens=1, table_stride=1000, max_len=100000))
+    for call, kw in ((decode, long), (prompt, long), (sample, {})):
+        lib.fake_reset(1)
+        assert call(lib, **kw) == -4
+        assert lib.fake_launches() == 0 and lib.fake_ws() > 0
+        lib.fake_reset(0)
+        assert call(lib, **kw) == 0 and lib.fake_launches() > 1
+
+
+def test_workspace_and_launches_follow_the_batch(lib):
+    """One part needs neither workspace nor a second launch; sampling runs many
+    rows in launches of 512."""
+    for call in (decode, prompt):
+        lib.fake_reset(0)
+        assert call(lib, b=batch(n_seqs=1, n_tokens=1, max_len=60)) == 0 and lib.fake_launches() == 1
+    lib.fake_reset(0)
+    assert sample(lib, rows=512, vocab=50257, stride=50257) == 0
+    one, ws = lib.fake_launches(), lib.fake_ws()
+    lib.fake_reset(0)
+    assert sample(lib, rows=1025, vocab=50257, stride=50257) == 0
+    assert lib.fake_launches() == 3 * one and lib.fake_ws() == ws < 64 << 20
