@@ -5,6 +5,8 @@
 #include <algorithm>
 #include <type_traits>
 
+#include <utility>
+
 #include "gq_paged.h"
 
 namespace {
@@ -74,6 +76,21 @@ __device__ __forceinline__ void swap_halves(float &a, float &b) {
   const uint32_t x = w[0], y = w[1]; /* a bit cast of w[1] itself would read w[0] */
   a = __builtin_bit_cast(float, x), b = __builtin_bit_cast(float, y);
 }
+/* lane J's value of the lane's row of 16, an operand's modifier */
+template <int J>
+__device__ __forceinline__ float of_row(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x150 + J, 0xf, 0xf, true));
+}
+/* f(0) .. f(N - 1) of compile-time numbers */
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each_of(F f) {
+  each_of(f, std::make_integer_sequence<int, N>{});
+}
+
 /* the larger of a lane's value and that of the lane 32 away */
 __device__ __forceinline__ float max_halves(float v) {
   float w = v;
@@ -106,10 +123,11 @@ __device__ __forceinline__ void pin(gq_bf16x8 &v, float &f) {
  * accuracy: bf16 values and int8 codes are exact there (the scales multiply
  * scores and probabilities), and an fp32 operand is split into three bf16
  * numbers that sum to it, of whose products those not below 2^-24 are kept:
- * three over a bf16 or int8 cache, six over an fp32 one.  bf16 queries, whose
- * results are bf16, take probabilities rounded to bf16 and an fp32 or int8
- * cache's values likewise: as exact as the queries themselves, for one product,
- * and for int8 without 64 products by scales a lane and block (2.5 -> 1.8 us).
+ * three over a bf16 or int8 cache, six over an fp32 one.  bf16 queries take
+ * probabilities rounded to bf16, like the results, and are exact themselves: one
+ * product, or two over an fp32 cache, whose values are two bf16 numbers there
+ * (2^-17).  With its values and int8 ones rounded to one, results are 0.0039 off
+ * in the mean for 0.0021, most of it by K.
  *
  * Keys that do not exist are masked, and their V zeros in LDS, so that what stale
  * memory holds cannot reach a sum.  So are infinities and NaN of V in the blocks that
@@ -121,15 +139,14 @@ __device__ __forceinline__ void pin(gq_bf16x8 &v, float &f) {
 template <int CT, int XT, int HD, int RG, int KH>
 __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_kernel(AttArgs a) {
   static_assert(RG * KH * GQ_WAVE == kPThreads, "eight waves");
-  constexpr int NX = XT == GQ_F32 ? 3 : 1, NK = NX == 3 && CT == GQ_F32 ? 3 : 1;
-  constexpr int NP = NX * NK == 9 ? 6 : NX; /* partial products */
+  constexpr int NX = XT == GQ_F32 ? 3 : 1, NK = CT != GQ_F32 ? 1 : NX == 3 ? 3 : 2;
+  constexpr int NP = NX * NK == 9 ? 6 : NX * NK; /* partial products */
   /* their planes of K or V and of Q or P, the small ones first */
-  constexpr int kA[3][6] = {{0}, {0, 0, 0}, {1, 2, 0, 1, 0, 0}}, kB[3][6] = {{0}, {2, 1, 0}, {1, 0, 2, 0, 1, 0}};
-  constexpr int W = NP == 6 ? 2 : NP == 3 ? 1 : 0;
-  constexpr int NB = NK == 1 ? 2 : 1;        /* blocks in LDS */
-  constexpr bool PIPE = NX == 1;
-  constexpr bool CODES = CT == GQ_I8_ROWS && NX == 3; /* int8 codes in LDS, scales apart; else values */
-  constexpr bool VALUES = CT == GQ_I8_ROWS && NX == 1;
+  constexpr int kA[4][6] = {{0}, {1, 0}, {0, 0, 0}, {1, 2, 0, 1, 0, 0}}, kB[4][6] = {{0}, {0, 0}, {2, 1, 0}, {1, 0, 2, 0, 1, 0}};
+  constexpr int W = NP == 6 ? 3 : NP - 1;
+  constexpr int NB = NK < 3 ? 2 : 1;         /* blocks in LDS */
+  constexpr bool PIPE = NP == 1;
+  constexpr bool CODES = CT == GQ_I8_ROWS;   /* in LDS, the scales apart */
   constexpr int EB = pgd_bytes(CT);
   constexpr int NO = HD / 8;                 /* octets of a K row */
   constexpr int NSL = HD / 16, ND = HD / 32; /* dim slices of S^T, dim tiles of O^T */
@@ -137,7 +154,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   constexpr int KPL = kKeys * HD * 2;        /* bytes of one plane */
   constexpr int KI = kKeys * NO / kPThreads; /* K octets a thread */
   constexpr int KPP = kPThreads / NO;        /* keys a pass of them */
-  constexpr int KW = 2 * EB + VALUES, VW = EB + VALUES;
+  constexpr int KW = 2 * EB, VW = EB;
   constexpr int VTH = 16 * HD / 4;           /* threads with four keys x four dims of V */
   constexpr int NQ = NX == 3 ? 2 : 1;        /* planes of Q in registers; the third in LDS */
   constexpr int QLO = NB * 2 * NK * KPL, SCL = QLO + (NX == 3 ? RG * NSL * 1024 : 0);
@@ -191,7 +208,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
    * page. */
   const int ko = tid % NO, kk = tid / NO, vd = tid % (HD / 4), va = tid / (HD / 4);
   const bool vtask = VTH == kPThreads || tid < VTH;
-  uint32_t kr[KI][KW], vr[4][VW]; /* raw dwords, and the scales of VALUES */
+  uint32_t kr[KI][KW], vr[4][VW]; /* raw dwords */
   float sc = 0.f;                     /* int8: the scale of key `lane`, K's in wave 0 and V's in wave 1 */
   const int ps = (1 << a.c.lg) - 1;
   uint32_t koff[KI]; /* within a page's rows for the head, from the block's first slot */
@@ -218,7 +235,6 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     for (int i = 0; i < KI; i++) {
       const size_t at = rows(b, kk + KPP * i);
       const uint8_t *kp = a.c.k + at * (size_t)(HD * EB);
-      if constexpr (VALUES) kr[i][2] = gld<uint32_t>(a.c.ks + at + ((kk + KPP * i) & ps));
       if constexpr (EB == 1) {
         const uint2 w = gld<uint2>(kp + koff[i]);
         kr[i][0] = w.x, kr[i][1] = w.y;
@@ -235,10 +251,6 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     if (vtask) {
       const size_t at = rows(b, 4 * va);
       const uint8_t *vp = a.c.v + at * (size_t)(HD * EB);
-      if constexpr (VALUES) {
-        const uint4 d = gld<uint4>(a.c.vs + at + ((4 * va) & ps));
-        vr[0][1] = d.x, vr[1][1] = d.y, vr[2][1] = d.z, vr[3][1] = d.w;
-      }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         if constexpr (EB == 1) {
@@ -280,14 +292,6 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         lst<uint4>(smem, at, make_uint4(kr[i][0], kr[i][1], kr[i][2], kr[i][3]));
       } else if constexpr (CODES) {
         lst<gq_bf16x8>(smem, at, codes8(kr[i][0], kr[i][1]));
-      } else if constexpr (VALUES) {
-        const float d = __builtin_bit_cast(float, kr[i][2]);
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = i8f(kr[i][e >> 2], e & 3) * d;
-        gq_bf16x8 p[1];
-        split8<1>(x, p);
-        lst<gq_bf16x8>(smem, at, p[0]);
       } else {
         float x[8];
 #pragma unroll
@@ -317,7 +321,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       /* added to an exponent of ones, one in its last place carries; fp32 values
        * that are to be bf16: from those on that round to an infinity */
       constexpr uint32_t ex = CT == GQ_BF16 ? 0x7f807f80u : 0x7fffffffu, top = CT == GQ_BF16 ? 0x80008000u : 0x80000000u;
-      constexpr uint32_t one = CT == GQ_BF16 ? 0x00800080u : CT == GQ_F32 && NK == 1 ? 0x00808000u : 0x00800000u;
+      constexpr uint32_t one = CT == GQ_BF16 ? 0x00800080u : CT == GQ_F32 ? 0x00808000u : 0x00800000u;
       uint32_t bad = 0;
       if constexpr (CODES) {
         bad = wv == 1 ? (__builtin_bit_cast(uint32_t, sc) & ex) + one : 0u;
@@ -325,7 +329,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-          for (int e = VALUES ? 1 : 0; e < VW; e++) bad |= (vr[i][e] & ex) + one;
+          for (int e = 0; e < VW; e++) bad |= (vr[i][e] & ex) + one;
       }
       if (__ballot((bad & top) != 0)) {
         odd = 1;
@@ -335,7 +339,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
           for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int e = VALUES ? 1 : 0; e < VW; e++) {
+            for (int e = 0; e < VW; e++) {
               const uint32_t c = ((vr[i][e] & ex) + one) & top;
               vr[i][e] &= ~(CT == GQ_BF16 ? (c >> 15) * 0xffffu : c ? ~0u : 0u);
             }
@@ -355,10 +359,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         } else if constexpr (CT == GQ_I8_ROWS) {
           float x[4];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            x[i] = i8f(vr[i][0], j);
-            if constexpr (VALUES) x[i] *= __builtin_bit_cast(float, vr[i][1]);
-          }
+          for (int i = 0; i < 4; i++) x[i] = i8f(vr[i][0], j);
           lst<uint2>(smem, at, make_uint2(pgd_pack(x[0], x[1]), pgd_pack(x[2], x[3])));
         } else {
           float x[4];
@@ -407,19 +408,33 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       }
     }
   };
-  /* int8: times K's scales, in units of log 2; keys that do not exist or lie past
-   * the row's position: -infinity */
+  /* int8: scores 4 c .. + 3 times K's scales (ring b & 3), in units of log 2, or
+   * the probabilities times V's (ring 4 + buffer).  Lane j of each row of 16
+   * holds the scale of the lanes' score j, where LDS would return all 16 to every
+   * lane: 512 tokens at 7500, 260 us by 16-byte reads, 231 so. */
+  struct Scales {
+    float d[KT];
+  };
+  auto scales = [&](int ring) {
+    Scales s{};
+    if constexpr (CODES)
+#pragma unroll
+      for (int t = 0; t < KT; t++)
+        s.d[t] = lld<float>(smem, SCL + (ring * kKeys + 32 * (kh + t) + 8 * (lane >> 2 & 3) + 4 * h + (lane & 3)) * 4);
+    return s;
+  };
+  auto times = [&](const Scales &s, gq_f32x16 (&st)[KT], auto c) {
+    if constexpr (CODES)
+      each_of<4>([&](auto i) {
+        constexpr int e = 4 * (c() % 4) + i();
+        st[c() / 4][e] *= of_row<e>(s.d[c() / 4]);
+      });
+  };
+  /* keys that do not exist or lie past the row's position: -infinity */
   auto mask = [&](int b, gq_f32x16 (&st)[KT]) {
     const int key0 = b * kKeys + 32 * kh, ok = exists(b);
 #pragma unroll
     for (int t = 0; t < KT; t++) {
-      if constexpr (CODES) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const float4 d = lld<float4>(smem, SCL + ((b & 3) * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
-          st[t][e] *= d.x, st[t][e + 1] *= d.y, st[t][e + 2] *= d.z, st[t][e + 3] *= d.w;
-        }
-      }
       if (ok != 15 || key0 + 32 * t + 31 > wlo) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
@@ -434,6 +449,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   bool rescale;
   /* the probabilities of masked scores, with V's scales for int8 */
   auto softmax = [&](int buf, gq_f32x16 (&st)[KT]) {
+    const Scales dv = scales(4 + buf);
     float mb = -INFINITY;
 #pragma unroll
     for (int t = 0; t < KT; t++)
@@ -453,13 +469,9 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         st[t][e] = __builtin_amdgcn_exp2f(CODES ? st[t][e] - ms : __builtin_fmaf(st[t][e], a.scale, -ms));
         l += st[t][e];
       }
-      if constexpr (CODES) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const float4 d = lld<float4>(smem, SCL + ((4 + buf) * kKeys + 32 * (kh + t) + 2 * e + 4 * h) * 4);
-          st[t][e] *= d.x, st[t][e + 1] *= d.y, st[t][e + 2] *= d.z, st[t][e + 3] *= d.w;
-        }
-      }
+      each_of<4 * KT>([&](auto c) {
+        if (c() / 4 == t) times(dv, st, c);
+      });
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         float x[8];
@@ -526,6 +538,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       }
       __syncthreads();
       scores(b0 & 1, sa);
+      const Scales dk = scales(b0 & 3);
+      each_of<4 * KT>([&](auto c) { times(dk, sa, c); });
       __syncthreads(); /* K of block 0 has been read */
       /* before it K of b and b + 1 and V of b are in LDS, K of b + 2 and V of b + 1
        * in registers.  Written in the order in which it is to run: four LDS
@@ -534,6 +548,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       auto body = [&](int b, gq_f32x16 (&cur)[KT], gq_f32x16 (&next)[KT]) {
         constexpr int N = KT * NSL, J = 4 * KT, N2 = 2 * KT * ND, A = 4; /* A operands ahead */
         mask(b, cur);
+        const Scales dv = scales(4 + (b & 1));
         const uint32_t kat = (uint32_t)(((b + 1) & 1) * 2 * KPL) + kbase, vat = (uint32_t)((b & 1) * 2 * KPL) + vbase;
         auto kop = [&](int i) { return lld<gq_bf16x8>(smem, (kat ^ (32 * (i / KT))) + 32 * (i % KT) * HD * 2); };
         auto vop = [&](int i) {
@@ -543,8 +558,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
         for (int i = 0; i < A; i++) w[i] = kop(i);
         float ms = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
+        each_of<N>([&](auto I) {
+          constexpr int i = I;
           __builtin_amdgcn_sched_barrier(0);
           next[i % KT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[i % A], q[i / KT][0], i < KT ? gq_f32x16{} : next[i % KT], 0, 0, 0);
           if (i + A < N) w[i % A] = kop(i + A);
@@ -555,21 +570,22 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
               for (int e = 0; e < 16; e++) mb = fmaxf(mb, cur[t][e]);
             mb = max_halves(mb);
-            mb *= a.scale;
+            if constexpr (!CODES) mb *= a.scale;
             const float mn = fmaxf(m, mb);
             ms = mn == -INFINITY ? 0.f : mn;
             alpha = __builtin_amdgcn_exp2f(m - ms);
             rescale = __ballot(mn > m) != 0;
             m = mn, l *= alpha;
           }
-#pragma unroll
-          for (int c = (i - 1) * J / (N - 1); i && c < i * J / (N - 1); c++) { /* scores 4 c .. + 3 */
-            const int t = c / 4, e0 = 4 * (c % 4);
+          each_of<J>([&](auto c) { /* scores 4 c .. + 3 */
+            if constexpr (i == 0 || c() < (i - 1) * J / (N - 1) || c() >= i * J / (N - 1)) return;
+            constexpr int t = c() / 4, e0 = 4 * (c() % 4);
 #pragma unroll
             for (int e = e0; e < e0 + 4; e++) {
-              cur[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(cur[t][e], a.scale, -ms));
+              cur[t][e] = __builtin_amdgcn_exp2f(CODES ? cur[t][e] - ms : __builtin_fmaf(cur[t][e], a.scale, -ms));
               l += cur[t][e];
             }
+            times(dv, cur, c);
             if (c & 1) {
               float x[8];
 #pragma unroll
@@ -577,8 +593,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
               split8<1>(x, pr[c / 2]);
               pin(pr[c / 2][0], l); /* here and not where they are used */
             }
-          }
-        }
+          });
+        });
         __builtin_amdgcn_sched_barrier(0);
         stagek(min(b + 2, bl), b & 1, kr, sc), stagev(min(b + 1, bl), (b + 1) & 1, vr, sc);
         loadk(min(b + 3, bl), kr), loads(min(b + 3, bl), 0, sc);
@@ -589,14 +605,18 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
             for (int e = 0; e < 16; e++) o[d][e] *= alpha;
         }
+        const Scales dk = scales((b + 1) & 3);
 #pragma unroll
         for (int i = 0; i < A; i++) w[i] = vop(i);
-#pragma unroll
-        for (int i = 0; i < N2; i++) {
+        each_of<N2>([&](auto I) {
+          constexpr int i = I;
           __builtin_amdgcn_sched_barrier(0);
           o[i % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[i % A], pr[i / ND][0], o[i % ND], 0, 0, 0);
           if (i + A < N2) w[i % A] = vop(i + A);
-        }
+          each_of<J>([&](auto c) {
+            if constexpr (c() >= i * J / N2 && c() < (i + 1) * J / N2) times(dk, next, c);
+          });
+        });
         __builtin_amdgcn_sched_barrier(0);
         turn(b + 1);
         __syncthreads();
@@ -613,6 +633,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       if (b * kKeys + 32 * kh > whi) return; /* none of this wave's rows sees any (uniform) */
       gq_f32x16 st[KT];
       scores(buf, st);
+      const Scales dk = scales(b & 3);
+      each_of<4 * KT>([&](auto c) { times(dk, st, c); });
       mask(b, st);
       softmax(buf, st);
       output(buf);
@@ -667,7 +689,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
         if constexpr (CT == GQ_F32) x = gld<float>((const float *)a.c.v + i);
         else if constexpr (CT == GQ_BF16) x = pgd_lo(gld<uint16_t>((const uint16_t *)a.c.v + i));
         else x = (float)*(const GQ_GLOBAL int8_t *)(a.c.v + i) * gld<float>(a.c.vs + at);
-        if constexpr (NX == 1) x = pgd_lo(pgd_pack(x, x));
+        if constexpr (CT == GQ_F32) x = pgd_lo(pgd_pack(x, x));
         if (u <= cpos && (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) == 0x7f800000u) o[d][e] += x;
         __builtin_amdgcn_sched_barrier(0); /* one load at a time: no registers beside the outputs */
       }
