@@ -411,7 +411,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
   /* int8: scores 4 c .. + 3 times K's scales (ring b & 3), in units of log 2, or
    * the probabilities times V's (ring 4 + buffer).  Lane j of each row of 16
    * holds the scale of the lanes' score j, where LDS would return all 16 to every
-   * lane: 512 tokens at 7500, 260 us by 16-byte reads, 231 so. */
+   * lane: 4 chunks of up to 512 tokens at up to 7500 260 us by 16-byte reads, 229
+   * so. */
   struct Scales {
     float d[KT];
   };
@@ -805,8 +806,8 @@ int launch_hd(const AttArgs &a, int hd, const PromptShape &f, hipStream_t s) {
 PromptShape gq_paged_prompt_shape(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu) {
   const bool f = xtype == GQ_F32, wide = head_dim > 64;
   const int t = cache == GQ_F32 ? 0 : cache == GQ_BF16 ? 1 : 2;
-  constexpr double kTau[2][3][3] = {{{1.31, 1.29, 1.35}, {0.94, 0.92, 0.95}, {2.42, 1.53, 1.80}},  /* head_dim 64: bf16 queries in 256 and 128 rows, fp32 */
-                                    {{1.98, 1.80, 1.90}, {1.58, 1.31, 1.40}, {5.66, 3.26, 3.39}}}; /* 128 */
+  constexpr double kTau[2][3][3] = {{{1.95, 1.32, 1.69}, {1.34, 0.97, 1.31}, {2.42, 1.53, 1.80}},  /* head_dim 64: bf16 queries in 256 and 128 rows, fp32 */
+                                    {{3.10, 1.77, 2.28}, {2.29, 1.31, 1.55}, {5.66, 3.49, 3.61}}}; /* 128 */
   const double fix = (f ? 5.0 : 10.0) * (wide ? 1.0 : 0.3);
   const int seqs = std::min(a.b.n_seqs, a.b.n_tokens), each = (a.b.n_tokens + seqs - 1) / seqs;
   const int nblk = std::max(1, (a.b.max_len + kKeys - 1) / kKeys);
