@@ -802,10 +802,11 @@ int launch_hd(const AttArgs &a, int hd, const PromptShape &f, hipStream_t s) {
  * number of new tokens alone, and takes the sequences for equally long.
  *
  * tau: one tile of 64 tokens over 8192 positions (32 heads over 8).  The other
- * constants are fitted to 300 launches timed with every choice (1 to 8
- * sequences, 1 to 2000 new tokens at 0 to 8000, head groups of 1 to 8): the rule's
- * choices take 2.5% more than the best ones together, 7% more for the worst in
- * ten; one part and 256 rows always, up to five times as long. */
+ * constants were fitted to launches timed with every choice (1 to 8 sequences, 1
+ * to 2000 new tokens at 0 to 8000, head groups of 1 to 8): over 170 others the
+ * rule's choices take 3% more than the best ones together, 5% more for the worst
+ * in ten; one part and 256 rows always, up to five times as long.
+ */
 PromptShape gq_paged_prompt_shape(const AttArgs &a, int cache, int xtype, int head_dim, int n_cu) {
   const bool f = xtype == GQ_F32, wide = head_dim > 64;
   const int t = cache == GQ_F32 ? 0 : cache == GQ_BF16 ? 1 : 2;
