@@ -280,7 +280,11 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
   int bid = blockIdx.x;
   const int g = bid % a.c.n_kv;
   bid /= a.c.n_kv;
-  const int part = bid % a.nch, item = bid / a.nch;
+  /* Workgroups go round the chip's engines in turn: with parts in the same order
+   * for every sequence, the ones that shorter sequences lack leave the same
+   * engines idle (128 sequences to 2000: 147 us, 116 with the order turned; 64 to
+   * 8192: 202, 193). */
+  const int item = bid / a.nch, part = (int)(((unsigned)bid + item + item / 2) % (unsigned)a.nch);
   /* sequence, row and length */
   const int s = item;
   int row, len;
