@@ -54,7 +54,10 @@ __device__ __forceinline__ int quant(float y, float d) {
 /* Where the rows of a wave are: U times RPW of the `per` rows of each packed
  * token, one of them this lane's.  Rows are counted in tiles of 16 tokens, token
  * after token for one head and then the next head: a wave's rows are neighbours
- * in a page, their scales too. */
+ * in a page, their scales too.  Memory bounds both kernels on long batches: 8122
+ * tokens of 32 + 16 bf16 rows appended in 49 us (4.3 TB/s of reads and writes),
+ * 32000 int8 rows of 8 heads read as fp32 in 83 (4.0); 32 tokens take 5.7 and 4.1,
+ * three dependent trips (sequence, page, rows). */
 constexpr int kRowTile = 16;
 template <int U>
 struct Rows {
@@ -264,7 +267,13 @@ __device__ __forceinline__ bool decode_row(const AttArgs &a, int s, int &row, in
  * int8 codes are exact in bf16; K's scale multiplies the score, V's the
  * probability.  fp32 caches use the fp32 matrix instructions, which need no
  * transposition (one key a step).  Keys that do not exist are masked, and V's
- * rows there are zeroed: what stale memory holds cannot reach a sum. */
+ * rows there are zeroed: what stale memory holds cannot reach a sum.
+ *
+ * The cache's bytes bound it: 64 sequences of up to 8192 positions (bf16, 32
+ * heads over 8 of 128, 998 MB) 175 us with the merge, 5.7 TB/s where a copy
+ * reaches 5.2; one of 131072 (int8, 277 MB) 51 us.  One of 301 takes 7.2 us: a
+ * launch and four dependent trips to memory.  Eight waves a workgroup were slower
+ * (64 sequences 250 us for 207 then). */
 template <int CT, int XT, int HD>
 __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
   constexpr int NW = kThreads / GQ_WAVE;
