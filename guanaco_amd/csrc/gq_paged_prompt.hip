@@ -686,8 +686,8 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     const uint4 f = lld<uint4>(smem, ODD), f1 = lld<uint4>(smem, ODD + 16);
     odd = (uint32_t)__builtin_amdgcn_readfirstlane((int)(f.x | f.y | f.z | f.w | f1.x | f1.y | f1.z | f1.w));
   }
-  for (int u = b0 * kKeys; odd && u < min(b1 * kKeys, pmax + 1); u++) {
-    const int page = partial(u / kKeys) && (KH == 1 || (u >> 5 & 1) == kh) ? pgd_page_u(a.c, a.b, s, u) : -1;
+  for (int u = max(b0, (pmin + 1) / kKeys) * kKeys; odd && u < min(b1 * kKeys, pmax + 1); u++) { /* partial blocks */
+    const int page = (KH == 1 || (u >> 5 & 1) == kh) ? pgd_page_u(a.c, a.b, s, u) : -1;
     if (page < 0) continue;
     const size_t at = pgd_row(a.c, page, g, u & ps);
 #pragma unroll
