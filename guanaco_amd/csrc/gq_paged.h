@@ -101,6 +101,13 @@ __device__ __forceinline__ void pgd_store8(void *base, size_t at, const float (&
   }
 }
 
+/* stores past the caches (the `nt` policy): whole lines that no wave reads again */
+template <class T>
+__device__ __forceinline__ void gst_nt(void *p, T v) {
+  typedef typename gq_native<sizeof(T)>::type N;
+  __builtin_nontemporal_store(__builtin_bit_cast(N, v), (GQ_GLOBAL N *)p);
+}
+
 /* byte i of a dword as a signed integer */
 __device__ __forceinline__ float i8f(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 

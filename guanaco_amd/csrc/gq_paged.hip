@@ -56,8 +56,11 @@ __device__ __forceinline__ int quant(float y, float d) {
  * after token for one head and then the next head: a wave's rows are neighbours
  * in a page, their scales too.  Memory bounds both kernels on long batches: 8122
  * tokens of 32 + 16 bf16 rows appended in 49 us (4.3 TB/s of reads and writes),
- * 32000 int8 rows of 8 heads read as fp32 in 83 (4.0); 32 tokens take 5.7 and 4.1,
- * three dependent trips (sequence, page, rows). */
+ * 32000 int8 rows of 8 heads read as fp32 in 49 (6.7 TB/s, four fifths of it
+ * writes); 32 tokens take 5.7 and 4.1, three dependent trips (sequence, page,
+ * rows).  Rows read are stored past the caches (83 us if not).  Rows appended are
+ * not, since attention reads them next: the append would take 44 us, reading 33 MB of
+ * them back 17 instead of 14. */
 constexpr int kRowTile = 16;
 template <int U>
 struct Rows {
@@ -112,16 +115,22 @@ __device__ __forceinline__ void load_row(const void *base, size_t at, int sub, f
     }
   }
 }
-template <int T, bool SPLIT, int HD>
+/* AWAY: past the caches */
+template <int T, bool SPLIT, int HD, bool AWAY>
 __device__ __forceinline__ void store_row(void *base, size_t at, int sub, const float (&x)[8]) {
+  const auto put = [](auto *p, auto v) {
+    if constexpr (AWAY) gst_nt(p, v);
+    else gst(p, v);
+  };
   if constexpr (!SPLIT) {
-    pgd_store8<T>(base, at + 8 * sub, x);
+    static_assert(T == GQ_BF16, "fp32 rows are split");
+    put((uint16_t *)base + at + 8 * sub, make_uint4(pgd_pack(x[0], x[1]), pgd_pack(x[2], x[3]), pgd_pack(x[4], x[5]), pgd_pack(x[6], x[7])));
   } else {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
       const size_t p = at + i * (HD / 2) + 4 * sub;
-      if constexpr (T == GQ_F32) gst<float4>((float *)base + p, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
-      else gst<uint2>((uint16_t *)base + p, make_uint2(pgd_pack(x[4 * i], x[4 * i + 1]), pgd_pack(x[4 * i + 2], x[4 * i + 3])));
+      if constexpr (T == GQ_F32) put((float *)base + p, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+      else put((uint16_t *)base + p, make_uint2(pgd_pack(x[4 * i], x[4 * i + 1]), pgd_pack(x[4 * i + 2], x[4 * i + 3])));
     }
   }
 }
@@ -163,13 +172,13 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
       }
     }
     if (isq) {
-      store_row<XT, SPLIT, HD>(a.q_out, (size_t)t * a.qos + (size_t)h * HD, sub, x);
+      store_row<XT, SPLIT, HD, false>(a.q_out, (size_t)t * a.qos + (size_t)h * HD, sub, x);
       continue;
     }
     const size_t row = pgd_row(a.c, o.page[u], h, p & ((1 << a.c.lg) - 1));
     uint8_t *pool = isk ? a.c.k : a.c.v;
     if constexpr (CT != GQ_I8_ROWS) {
-      store_row<CT, SPLIT, HD>(pool, row * HD, sub, x);
+      store_row<CT, SPLIT, HD, false>(pool, row * HD, sub, x);
     } else {
       float m = 0.f;
       bool bad = false;
@@ -231,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
   for (int u = 0; u < U; u++) {
     if (o.t[u] < 0) continue;
     const bool isk = o.j[u] < a.c.n_kv;
-    store_row<XT, SPLIT, HD>(isk ? a.k : a.v, (size_t)o.t[u] * (isk ? a.ks : a.vs) + (size_t)(isk ? o.j[u] : o.j[u] - a.c.n_kv) * HD, sub, x[u]);
+    store_row<XT, SPLIT, HD, true>(isk ? a.k : a.v, (size_t)o.t[u] * (isk ? a.ks : a.vs) + (size_t)(isk ? o.j[u] : o.j[u] - a.c.n_kv) * HD, sub, x[u]);
   }
 }
 
