@@ -403,7 +403,7 @@ def test_values_that_are_no_numbers_stay_in_their_future(ctx, case, cache, xt):
             if cache == I8:
                 w.pools[which][1][g, head, o] = np.nan
             else:
-                w.pools[which][0][g, head, o, dim] = enc(v, cache)
+                w.pools[which][0][g, head, o, dim] = enc(np.array([v]), cache)[0]
             w.upload(ctx, H)
             got = attend(ctx, w, nh, xt, "paged_prompt_dev")[1]
             w.free()
