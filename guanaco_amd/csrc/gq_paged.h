@@ -150,6 +150,27 @@ struct AttArgs {
   float scale;    /* log2(e) / sqrt(head_dim) */
 };
 
+/* What a workgroup of the prompt kernel has in LDS: blocks of 64 keys, 32 RG
+ * query rows, a wave with 64 / KH keys of every block. */
+constexpr int kKeys = 64;
+template <int CT, int XT, int HD, int RG, int KH>
+struct PromptLds {
+  /* bf16 planes of Q or P and of K or V */
+  static constexpr int NX = XT == GQ_F32 ? 3 : 1, NK = CT != GQ_F32 ? 1 : NX == 3 ? 3 : 2;
+  static constexpr int NB = NK < 3 ? 2 : 1;       /* blocks */
+  static constexpr bool CODES = CT == GQ_I8_ROWS; /* the scales apart */
+  static constexpr int KPL = kKeys * HD * 2;      /* bytes of one plane */
+  static constexpr int QLO = NB * 2 * NK * KPL;   /* the third plane of Q; the others are in registers */
+  static constexpr int SCL = QLO + (NX == 3 ? RG * (HD / 16) * 1024 : 0);
+  static constexpr int USED = SCL + (CODES ? (4 + NB) * kKeys * 4 : 0); /* scales: four blocks of K's, NB of V's */
+  /* the halves' exchange at the end, from 0 on: (m, l, O) of a lane */
+  static constexpr int EXCHANGE = KH == 2 ? RG * 64 * 4 * (HD / 32 * 16 + 2) : 0;
+  /* a flag per wave, read when other waves have begun the exchange: behind it */
+  static constexpr int ODD = USED > EXCHANGE ? USED : EXCHANGE;
+  static constexpr int BYTES = ODD + 32;
+  static_assert(ODD % 16 == 0 && BYTES <= 160 * 1024, "flags are read 16 bytes at a time; LDS of a CU");
+};
+
 /* gq_paged_prompt.hip: every new token's attention.  The shape of its launch:
  * rows of a tile, blocks of 64 keys a part, at most so many parts (more than
  * one: part_o and part_ml hold n_tokens rows), workgroups (0: too many). */

@@ -13,7 +13,7 @@ namespace {
 
 typedef float gq_f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kPThreads = 512, kKeys = 64;
+constexpr int kPThreads = 512;
 
 /* A tile of query rows: up to tpt new tokens of a sequence, from its t0-th on,
  * packed from row `row` on; p0 positions are before the sequence's first. */
@@ -145,29 +145,27 @@ __device__ __forceinline__ void pin(gq_bf16x8 &v, float &f) {
 template <int CT, int XT, int HD, int RG, int KH>
 __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void prompt_kernel(AttArgs a) {
   static_assert(RG * KH * GQ_WAVE == kPThreads, "eight waves");
-  constexpr int NX = XT == GQ_F32 ? 3 : 1, NK = CT != GQ_F32 ? 1 : NX == 3 ? 3 : 2;
+  typedef PromptLds<CT, XT, HD, RG, KH> Lds;
+  constexpr int NX = Lds::NX, NK = Lds::NK;
   constexpr int NP = NX * NK == 9 ? 6 : NX * NK; /* partial products */
   /* their planes of K or V and of Q or P, the small ones first */
   constexpr int kA[4][6] = {{0}, {1, 0}, {0, 0, 0}, {1, 2, 0, 1, 0, 0}}, kB[4][6] = {{0}, {0, 0}, {2, 1, 0}, {1, 0, 2, 0, 1, 0}};
   constexpr int W = NP == 6 ? 3 : NP - 1;
-  constexpr int NB = NK < 3 ? 2 : 1;         /* blocks in LDS */
+  constexpr int NB = Lds::NB;
   constexpr bool PIPE = NP == 1;
-  constexpr bool CODES = CT == GQ_I8_ROWS;   /* in LDS, the scales apart */
+  constexpr bool CODES = Lds::CODES;
   constexpr int EB = pgd_bytes(CT);
   constexpr int NO = HD / 8;                 /* octets of a K row */
   constexpr int NSL = HD / 16, ND = HD / 32; /* dim slices of S^T, dim tiles of O^T */
   constexpr int KT = 2 / KH;                 /* 32-key tiles of a wave's */
-  constexpr int KPL = kKeys * HD * 2;        /* bytes of one plane */
+  constexpr int KPL = Lds::KPL;
   constexpr int KI = kKeys * NO / kPThreads; /* K octets a thread */
   constexpr int KPP = kPThreads / NO;        /* keys a pass of them */
   constexpr int KW = 2 * EB, VW = EB;
   constexpr int VTH = 16 * HD / 4;           /* threads with four keys x four dims of V */
   constexpr int NQ = NX == 3 ? 2 : 1;        /* planes of Q in registers; the third in LDS */
-  constexpr int QLO = NB * 2 * NK * KPL, SCL = QLO + (NX == 3 ? RG * NSL * 1024 : 0);
-  constexpr int ODD = SCL + (CODES ? (4 + NB) * kKeys * 4 : 0);          /* scales: four blocks of K's, NB of V's */
-  constexpr int LDS = std::max(ODD + 32, /* a flag per wave */
-                               KH == 2 ? RG * 64 * 4 * (ND * 16 + 2) : 0);          /* the halves' exchange */
-  __shared__ __attribute__((aligned(16))) uint8_t smem_[LDS];
+  constexpr int QLO = Lds::QLO, SCL = Lds::SCL, ODD = Lds::ODD;
+  __shared__ __attribute__((aligned(16))) uint8_t smem_[Lds::BYTES];
   GQ_LDS uint8_t *smem = (GQ_LDS uint8_t *)smem_;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wv / KH, kh = wv % KH;
@@ -705,7 +703,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
       }
   }
   l += __shfl_xor(l, 32, 64);
-  if constexpr (KH == 2) { /* kh = 1 hands (m, l, O) to kh = 0 */
+  if constexpr (KH == 2) { /* kh = 1 hands (m, l, O) to kh = 0; slower waves may still read the flags */
     GQ_LDS float *x = (GQ_LDS float *)smem + rg * 64 * (ND * 16 + 2);
     if (kh == 1) {
       x[lane] = m, x[64 + lane] = l;
