@@ -40,9 +40,14 @@ __device__ __forceinline__ int pgd_seq_of(const PgdBatch &b, int t) {
 }
 
 /* Positions before the call's tokens.  None from max_len on exists, so that a
- * larger number says no more than max_len; the sum with a token's number then
- * stays within 31 bits (max_len and n_tokens are 2^30 at most). */
+ * larger number says no more than max_len; the sum with a token's number, 0 to
+ * n_tokens - 1, then stays within 31 bits (max_len and n_tokens are 2^30 at
+ * most).  With n_tokens itself it need not: pgd_len. */
 __device__ __forceinline__ int pgd_before(const PgdBatch &b, int pos) { return min(pos, b.max_len); }
+/* positions that exist once n tokens follow `before` ones (< 0: an idle slot) */
+__host__ __device__ __forceinline__ int pgd_len(int before, int n, int max_len) {
+  return before < 0 ? 0 : before < max_len - n ? before + n : max_len;
+}
 
 /* (row of the first new token, their number) of a sequence, s uniform in the
  * wave; none where the rows are not in the packed arrays */

@@ -250,9 +250,8 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
 __device__ __forceinline__ bool decode_row(const AttArgs &a, int s, int &row, int &len) {
   const int2 rn = pgd_rows(a.b, s);
   if (rn.y < 1) return false;
-  const int p0 = pgd_before(a.b, gq_sld<int>(a.b.pos + s));
   row = rn.x + rn.y - 1;
-  len = p0 < 0 ? 0 : min(p0 + rn.y, a.b.max_len);
+  len = pgd_len(gq_sld<int>(a.b.pos + s), rn.y, a.b.max_len);
   return true;
 }
 

@@ -34,7 +34,7 @@ __device__ __forceinline__ Tile find_tile(const PgdBatch &b, int tpt, int id) {
     if (!in) r0 = r1 = 0;
     int sq = q;
     if (cnt > 1) { /* lane i: the i-th longest */
-      const int len = in ? max(p0, 0) + (r1 - r0) : -1;
+      const int len = in ? pgd_len(p0, r1 - r0, b.max_len) : -1;
       int rank = 0;
       for (int i = 0; i < cnt; i++) {
         const int u = __builtin_amdgcn_readlane(len, i);

@@ -33,3 +33,5 @@ extern "C" int parts_prompt_lds(int *out) {
   n += lds_of_cache<GQ_BF16>(out + n);
   return n + lds_of_cache<GQ_I8_ROWS>(out + n);
 }
+
+extern "C" int parts_len(int before, int n, int max_len) { return pgd_len(before, n, max_len); }
