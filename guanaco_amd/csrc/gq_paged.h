@@ -141,6 +141,9 @@ __device__ __forceinline__ gq_bf16x8 codes8(uint32_t a, uint32_t b) {
                                                   pgd_pack(i8f(b, 0), i8f(b, 1)), pgd_pack(i8f(b, 2), i8f(b, 3))));
 }
 
+/* HIP counts a launch's threads in 32 bits */
+inline bool pgd_launchable(long long blocks, int threads) { return blocks * threads < (1ll << 32); }
+
 constexpr int kMaxG = 16; /* query heads per KV head */
 
 /* attention of new tokens over the cache */

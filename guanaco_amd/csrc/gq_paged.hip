@@ -669,11 +669,11 @@ void dispatch(int ct, int xt, int hd, F f) {
  * two waves a SIMD; below, a load each and more waves.  8122 tokens of 48 rows
  * with their read: 63 us against 72. */
 bool wide_rows(long long rows) { return rows >= 32768; }
-/* their workgroups; 0: more rows than they count */
+/* their workgroups; 0: more than a launch takes */
 unsigned row_blocks(long long tokens, int each, int hd, bool wide) {
   const long long rows = (tokens + kRowTile - 1) / kRowTile * kRowTile * each;
-  const long long per = wide ? kThreads / GQ_WAVE * kRowTile : kThreads / (hd / 8);
-  return rows < (1ll << 31) - per ? (unsigned)((rows + per - 1) / per) : 0u;
+  const long long per = wide ? kThreads / GQ_WAVE * kRowTile : kThreads / (hd / 8), blocks = (rows + per - 1) / per;
+  return pgd_launchable(blocks, kThreads) ? (unsigned)blocks : 0u;
 }
 
 /* the arguments of an attention over the cache: 0, a status, or 1 for nothing
@@ -751,7 +751,8 @@ extern "C" int gq_hip_paged_decode_dev(gq_ctx *c, const gq_pages *p, const gq_ba
   a.chunk = decode_chunk(b, p, ci.n_cu);
   a.nch = std::max(1, (b->max_len + a.chunk - 1) / a.chunk);
   const long long blocks = (long long)b->n_seqs * p->n_kv_heads * a.nch, rows = (long long)b->n_seqs * n_heads;
-  if (std::max(blocks, rows * (p->head_dim / 32)) >= (1ll << 31)) return gq_ctx_fail(c, -1, "paged decode: the batch passes a launch");
+  if (!pgd_launchable(blocks, kThreads) || (a.nch > 1 && !pgd_launchable(rows * (p->head_dim / 32), kThreads)))
+    return gq_ctx_fail(c, -1, "paged decode: the batch passes a launch");
   if (a.nch > 1) {
     a.part_o = (float *)gq_ctx_paged_ws(c, sizeof(float) * rows * a.nch * (p->head_dim + 2));
     if (!a.part_o) return -4;

@@ -750,14 +750,14 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 /* The parts of a row's keys, a workgroup per token: out = sum_c o_c 2^(m_c - M) /
  * sum_c l_c 2^(m_c - M), four dims of a head a thread. */
 template <int XT, int HD>
-__global__ __launch_bounds__(512) void prompt_merge_kernel(AttArgs a, int tpt) {
+__global__ __launch_bounds__(kPThreads) void prompt_merge_kernel(AttArgs a, int tpt) {
   const int row = blockIdx.x, s = __builtin_amdgcn_readfirstlane(pgd_seq_of(a.b, row));
   if (s >= a.b.n_seqs) return;
   const int2 rn = pgd_rows(a.b, s);
   if (row < rn.x || row >= rn.x + rn.y) return;
   const int parts = tile_blocks(a, pgd_before(a.b, gq_sld<int>(a.b.pos + s)), min((row - rn.x) / tpt * tpt + tpt, rn.y) - 1).y;
   if (parts <= 1) return; /* its one part has written the result */
-  for (int i = threadIdx.x; i < a.n_heads * (HD / 4); i += 512) {
+  for (int i = threadIdx.x; i < a.n_heads * (HD / 4); i += kPThreads) {
     const int qh = i / (HD / 4), dim = 4 * (i % (HD / 4));
     const size_t at = ((size_t)row * a.n_heads + qh) * a.nch;
     float M = -INFINITY;
@@ -784,7 +784,7 @@ __global__ __launch_bounds__(512) void prompt_merge_kernel(AttArgs a, int tpt) {
 template <int CT, int XT, int HD, int RG>
 int launch(const AttArgs &a, unsigned blocks, int tpt, hipStream_t s) {
   hipLaunchKernelGGL((prompt_kernel<CT, XT, HD, RG, 8 / RG>), dim3(blocks), dim3(kPThreads), 0, s, a);
-  if (a.nch > 1) hipLaunchKernelGGL((prompt_merge_kernel<XT, HD>), dim3(a.b.n_tokens), dim3(512), 0, s, a, tpt);
+  if (a.nch > 1) hipLaunchKernelGGL((prompt_merge_kernel<XT, HD>), dim3(a.b.n_tokens), dim3(kPThreads), 0, s, a, tpt);
   return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
@@ -825,7 +825,8 @@ PromptShape gq_paged_prompt_shape(const AttArgs &a, int cache, int xtype, int he
   for (int rows = f ? 128 : 256; rows >= 128; rows /= 2) {
     const int tpt = rows / a.G;
     const double w = (double)seqs * ((each + tpt - 1) / tpt) * a.c.n_kv, tau = kTau[wide][f ? 2 : rows == 128][t];
-    for (int k = 1; k <= std::min(16, nblk); k++) {
+    const int most = pgd_launchable(a.b.n_tokens, kPThreads) ? std::min(16, nblk) : 1; /* the merge's launch */
+    for (int k = 1; k <= most; k++) {
       const int span = (nblk + k - 1) / k;
       const double parts = std::max(1.0, mean / span), longest = fix + tau * span;
       const double load = w * (parts * fix + tau * mean) / n_cu;
@@ -835,7 +836,7 @@ PromptShape gq_paged_prompt_shape(const AttArgs &a, int cache, int xtype, int he
     }
   }
   const long long tiles = a.b.n_tokens / (best.rows / a.G) + seqs, blocks = tiles * a.c.n_kv * best.parts;
-  best.blocks = blocks < (1ll << 31) ? (unsigned)blocks : 0u;
+  best.blocks = pgd_launchable(blocks, kPThreads) ? (unsigned)blocks : 0u;
   return best;
 }
 
