@@ -605,14 +605,21 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(AttArgs a) {
  * 512).  One part, without the merge's launch of 3 us, where a sequence is
  * short (one of 256, bf16: 6.6 against 9.3; of 512: 11.1 against 9.9), or where
  * the sequences alone fill the chip (64 of 500: 20 against 32; 32 of 1000,
- * int8: 19.6 against 21.8). */
+ * int8: 19.6 against 21.8).
+ * At most 64 workgroups a CU, since the bound may be far above most lengths:
+ * every part costs a workgroup and workspace for its results, 34 MB then at four
+ * heads per KV head.  fp32 queries over bf16, 32 heads over 8 of 128, bound
+ * 131072: 128 sequences of 1000 104 us (343 without a limit, 116 at 128 a CU, 100
+ * at 32), one of 131072 among them 186 (414, 188, 286); 128 of up to 16384 742
+ * (791, 791, 727). */
 int decode_chunk(const gq_batch *b, const gq_pages *p, int n_cu) {
   const int row = 2 * p->head_dim * pgd_bytes(p->dtype), by = 256 * 1024 / row;
   const long long heads = (long long)b->n_seqs * p->n_kv_heads;
   const int whole = std::max(1, (b->max_len + 127) / 128) * 128;
   if (b->max_len <= std::min(384, 192 * 1024 / row) || (heads >= n_cu && b->max_len <= by)) return whole;
   const long long even = (heads * b->max_len / (2 * n_cu) + 127) / 128 * 128;
-  return (int)std::min<long long>({(long long)by, std::max<long long>(even, 128), (long long)whole});
+  const long long most = std::max(1ll, 64ll * n_cu / heads), least = ((b->max_len + most - 1) / most + 127) / 128 * 128;
+  return (int)std::min<long long>(std::max(std::min<long long>(by, std::max<long long>(even, 128)), least), whole);
 }
 
 /* ------------------------------------------------------------ entry points */

@@ -2,7 +2,7 @@
 (tests/test_paged_host.py's stand-in for the context and HIP)."""
 import pytest
 
-from test_paged_host import A, F32, BF16, append, batch, decode, lib, pages, prompt, read  # noqa: F401
+from test_paged_host import A, BF16, F32, I8, append, batch, decode, lib, pages, prompt, read  # noqa: F401
 
 BIG = dict(table_stride=1 << 20)
 
@@ -30,3 +30,16 @@ def test_launches_of_less_than_2_to_the_32_threads(lib, call, p, fits, past, kw)
     lib.fake_reset(0)
     assert call(lib, p, past, BF16, **kw) == -1
     assert lib.fake_launches() == 0 and lib.fake_error()
+
+
+@pytest.mark.parametrize("nkv,heads,hd,cache", [(8, 32, 128, BF16), (8, 32, 128, I8), (1, 16, 64, F32), (4, 4, 64, I8)])
+@pytest.mark.parametrize("seqs,max_len", [(1, 1 << 30), (16, 1 << 20), (128, 131072), (128, 32768), (1024, 1 << 20), (5000, 4096), (40000, 1000000)])
+def test_decode_workspace_is_bounded(lib, seqs, max_len, nkv, heads, hd, cache):  # noqa: F811
+    """A far bound on the length costs no more than 64 workgroups a CU (of 256)
+    and their results: parts are longer instead."""
+    lib.fake_reset(0)
+    p = pages(n_kv_heads=nkv, head_dim=hd, dtype=cache, page_size=1024, n_pages=1 << 20)
+    assert decode(lib, p, batch(n_seqs=seqs, n_tokens=seqs, max_len=max_len, table_stride=1 << 20, first=None), nh=heads) == 0, lib.fake_error()
+    most = max(64 * 256, seqs * nkv)
+    assert lib.fake_ws() <= most * (heads // nkv) * (hd + 2) * 4
+    assert lib.fake_blocks() <= most + seqs * heads * (hd // 32)
