@@ -29,8 +29,10 @@ struct GqDeviceGuard {
 };
 /* sets the context's error message and returns code */
 int gq_ctx_fail(gq_ctx *c, int code, const char *msg);
-/* the context's workspace of the paged entry points, at least so many bytes;
- * it only grows, behind the work that still uses it.  NULL: no memory. */
+/* the context's workspace of the paged entry points and the batch sampler, at
+ * least so many bytes, for the launches that follow at once: it grows behind the
+ * work that still uses it, and other requests that find no room take it back.
+ * NULL: no memory. */
 void *gq_ctx_paged_ws(gq_ctx *c, size_t bytes);
 
 /* ---- quantised matvec ----------------------------------------------------

@@ -313,19 +313,25 @@ static bool dense_drop(gq_ctx *c);
 static size_t dense_held(const gq_ctx *c);
 static void pf_drop(gq_ctx *c);
 static size_t pf_held(const gq_ctx *c);
-/* A request that finds no room takes back what prompts can do without if it
- * fits then: their workspaces, which the next one makes as the room allows,
- * and then the bf16 copies of the weights.  Want::prompt: the caller is a
+static void paged_drop(gq_ctx *c);
+/* A request that finds no room takes back what can be made again if it fits
+ * then: the prompts' workspaces, which the next one makes as the room allows,
+ * that of the paged entry points, and then the bf16 copies of the weights.  Want::prompt: the caller is a
  * prompt, whose workspaces are in use.  Want::optional: it can do without too;
  * nothing is taken back. */
 enum class Want { must, prompt, optional };
 static void *dev_alloc(gq_ctx *c, size_t bytes, Want want = Want::must) {
   void *p = try_malloc(bytes + kPad);
   const size_t ws = want == Want::must ? pf_held(c) : 0, copies = want != Want::optional ? dense_held(c) : 0;
+  const size_t paged = want != Want::optional ? c->paged_cap : 0;
   size_t fr = 0, tot = 0;
-  if (!p && ws + copies && hipMemGetInfo(&fr, &tot) == hipSuccess && bytes <= fr + ws + copies) {
+  if (!p && ws + paged + copies && hipMemGetInfo(&fr, &tot) == hipSuccess && bytes <= fr + ws + paged + copies) {
     if (ws) {
       pf_drop(c);
+      p = try_malloc(bytes + kPad);
+    }
+    if (!p && paged) {
+      paged_drop(c);
       p = try_malloc(bytes + kPad);
     }
     if (!p && copies && dense_drop(c)) p = try_malloc(bytes + kPad);
@@ -2219,10 +2225,14 @@ GqCtxInfo gq_ctx_info(const gq_ctx *c) { return GqCtxInfo{c->dev, c->n_cu, c->st
 
 int gq_ctx_fail(gq_ctx *c, int code, const char *msg) { return fail(c, code, "%s", msg); }
 
+static void paged_drop(gq_ctx *c) {
+  if (c->paged_ws) gq_hip_free(c, c->paged_ws); /* waits for the launches that still use it */
+  c->paged_ws = nullptr, c->paged_cap = 0;
+}
+
 void *gq_ctx_paged_ws(gq_ctx *c, size_t bytes) {
   if (c->paged_cap >= bytes) return c->paged_ws;
-  if (c->paged_ws) gq_hip_free(c, c->paged_ws); /* waits for the launches that still use it */
-  c->paged_cap = 0;
+  paged_drop(c);
   c->paged_ws = dev_alloc(c, bytes);
   if (c->paged_ws) c->paged_cap = bytes;
   return c->paged_ws;
