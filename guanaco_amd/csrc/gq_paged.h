@@ -144,6 +144,10 @@ __device__ __forceinline__ gq_bf16x8 codes8(uint32_t a, uint32_t b) {
 /* HIP counts a launch's threads in 32 bits */
 inline bool pgd_launchable(long long blocks, int threads) { return blocks * threads < (1ll << 32); }
 
+/* An output that an infinity or NaN of V has reached is NaN, whatever the order
+ * and the parts that its weight came in made of it: infinity here, NaN there. */
+__device__ __forceinline__ float pgd_finite(float y) { return __builtin_fmaf(y, 0.f, y); }
+
 constexpr int kMaxG = 16; /* query heads per KV head */
 
 /* attention of new tokens over the cache */

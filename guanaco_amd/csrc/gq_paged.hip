@@ -538,7 +538,7 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
     }
     const int qh = g * a.G + h;
     if (parts == 1) {
-      y = L == 0.f ? 0.f : y / L; /* nothing seen: zeros */
+      y = pgd_finite(L == 0.f ? y * 0.f : y / L); /* nothing seen: zeros */
       const size_t at = (size_t)row * a.os + (size_t)qh * HD + d;
       if constexpr (XT == GQ_F32) gst<float>((float *)a.out + at, y);
       else gst<uint16_t>((uint16_t *)a.out + at, (uint16_t)pgd_pack(y, y));
@@ -589,7 +589,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(AttArgs a) {
     float t = 0.f, l = 0.f;
 #pragma unroll 8
     for (int i = 0; i < 32; i++) t += sacc[i][tid], l += sL[i];
-    t = l == 0.f ? 0.f : t / l;
+    t = pgd_finite(l == 0.f ? t * 0.f : t / l);
     const size_t o = (size_t)row * a.os + (size_t)h * HD + 32 * dg + tid;
     if constexpr (XT == GQ_F32) gst<float>((float *)a.out + o, t);
     else gst<uint16_t>((uint16_t *)a.out + o, (uint16_t)pgd_pack(t, t));

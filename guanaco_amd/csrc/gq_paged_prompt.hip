@@ -677,7 +677,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
     }
   }
   /* The values of partial blocks that are no numbers, to the outputs of the rows
-   * that see them: times a weight above zero an infinity or NaN is the same. */
+   * that see them, which they make NaN (pgd_finite). */
   if (lane == 0) lst<uint32_t>(smem, ODD + 4 * wv, odd);
   __syncthreads();
   {
@@ -736,6 +736,7 @@ __global__ __launch_bounds__(kPThreads) __attribute__((amdgpu_waves_per_eu(2, 2)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         y[e] = o[d][8 * c + e] * inv, y[4 + e] = o[d][8 * c + 4 + e] * inv;
+        if (whole) y[e] = pgd_finite(y[e]), y[4 + e] = pgd_finite(y[4 + e]);
         swap_halves(y[e], y[4 + e]);
       }
       const int dim = 32 * d + 16 * c + 8 * h;
@@ -775,9 +776,10 @@ __global__ __launch_bounds__(kPThreads) void prompt_merge_kernel(AttArgs a, int 
       y.z = __builtin_fmaf(o.z, w, y.z), y.w = __builtin_fmaf(o.w, w, y.w);
     }
     const float inv = L == 0.f ? 0.f : 1.0f / L;
+    y.x = pgd_finite(y.x * inv), y.y = pgd_finite(y.y * inv), y.z = pgd_finite(y.z * inv), y.w = pgd_finite(y.w * inv);
     const size_t o = (size_t)row * a.os + (size_t)qh * HD + dim;
-    if constexpr (XT == GQ_F32) gst<float4>((float *)a.out + o, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
-    else gst<uint2>((uint16_t *)a.out + o, make_uint2(pgd_pack(y.x * inv, y.y * inv), pgd_pack(y.z * inv, y.w * inv)));
+    if constexpr (XT == GQ_F32) gst<float4>((float *)a.out + o, y);
+    else gst<uint2>((uint16_t *)a.out + o, make_uint2(pgd_pack(y.x, y.y), pgd_pack(y.z, y.w)));
   }
 }
 

@@ -483,8 +483,13 @@ int gq_hip_paged_decode_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *
  * sequence s over positions 0 .. pos[s] + t, whose rows are in the cache.
  * GQ_F32 queries keep fp32 accuracy throughout; with GQ_BF16 ones the
  * probabilities are rounded to bf16 before they meet V, and the values of a
- * GQ_F32 or GQ_I8_ROWS cache before they meet either.  An infinity or NaN in
- * the cache reaches the tokens that see its position and no others. */
+ * GQ_F32 or GQ_I8_ROWS cache before they meet either.
+ * Both attentions: an infinity or NaN in the cache reaches the tokens that see
+ * its position and no others.  Of V, or in the scale of its row, it makes their
+ * outputs in its dimension (the row's dimensions) NaN.  Of K it makes the score
+ * an infinity or NaN, and so all outputs of the head NaN unless the score is
+ * -infinity, which weighs nothing.  fp32 numbers that round to bf16's infinity
+ * (3.3962e38 and more) may count as infinite. */
 int gq_hip_paged_prompt_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
                             const void *q, int q_stride, void *out, int out_stride);
 
