@@ -640,7 +640,10 @@ int check_cache(gq_ctx *c, const gq_pages *p, const gq_batch *b, int xtype) {
     return gq_ctx_fail(c, -1, "paged: page_size is a power of two from 16 to 1024");
   if (b->n_seqs < 0 || b->n_tokens < 0) return gq_ctx_fail(c, -1, "paged: negative size of the batch");
   if (b->n_seqs && (!b->table || !b->pos || b->table_stride < 1 || b->max_len < 0)) return gq_ctx_fail(c, -1, "paged: incomplete batch");
-  if (b->max_len > (1 << 30) || b->n_tokens > (1 << 30)) return gq_ctx_fail(c, -1, "paged: max_len or n_tokens passes 2^30");
+  if (b->n_seqs && (((uintptr_t)b->table | (uintptr_t)b->pos | (uintptr_t)b->first) & 3))
+    return gq_ctx_fail(c, -1, "paged: table, pos or first is not 4-byte aligned");
+  if (b->max_len > (1 << 30) || b->n_tokens > (1 << 30) || b->n_seqs > (1 << 30))
+    return gq_ctx_fail(c, -1, "paged: max_len, n_tokens or n_seqs passes 2^30");
   if (!b->first && b->n_tokens < b->n_seqs) return gq_ctx_fail(c, -1, "paged: fewer rows than sequences");
   if (b->n_seqs && (long long)b->max_len > (long long)b->table_stride * p->page_size)
     return gq_ctx_fail(c, -5, "paged: max_len passes the page table");

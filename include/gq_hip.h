@@ -412,10 +412,12 @@ size_t gq_hip_prefill_copy_bytes(gq_ctx *ctx);
  * new token a sequence and of packed prompts, and sampling for a batch.  No
  * counterpart in the reference, which holds one sequence in one fp32 slab.
  *
- * All pointers are device memory of the context's GPU, 16-byte aligned, and
- * the caller's to keep (gq_hip_malloc, or any other allocation); calls are
- * asynchronous on the context's stream and hold nothing of their arguments
- * afterwards.  Lengths and pages are read on the device: a batch of the same
+ * All pointers are device memory of the context's GPU, 16-byte aligned (table,
+ * pos and first: 4-byte), and the caller's to keep (gq_hip_malloc, or any other
+ * allocation); calls are asynchronous on the context's stream and hold nothing
+ * of their arguments afterwards.  That stream waits for no other: what another
+ * one writes has to be there before the call, and gq_hip_sync says that a
+ * result is.  Lengths and pages are read on the device: a batch of the same
  * n_seqs, n_tokens and max_len runs through the same launches whatever they
  * say. */
 
@@ -441,7 +443,7 @@ typedef struct {
  * their number (0 is allowed).  first NULL: one token each, row s.  max_len: no
  * sequence is longer, its new tokens included; positions from there on do not
  * exist either.  It sizes launches and workspaces, so a close bound is faster.
- * max_len and n_tokens: 2^30 at most. */
+ * max_len, n_tokens and n_seqs: 2^30 at most. */
 typedef struct {
   const int32_t *table, *pos, *first;
   int n_seqs, table_stride, n_tokens, max_len;
@@ -459,7 +461,9 @@ typedef struct {
  * nearest even as if exact, within -127 .. 127; a row that holds an infinity or
  * NaN gets the scale NaN.  Tokens whose position does not exist are left out,
  * and their q_out rows left as they were.
- * 0; -1 bad argument; -5 max_len beyond the table's or rope's rows. */
+ * 0; -1 bad argument, or a batch past what a launch takes (2^32 threads); -4 the
+ * launch failed, or its workspace found no memory; -5 max_len beyond the table's
+ * or rope's rows.  So do the entry points below. */
 int gq_hip_paged_append_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
                             const void *q, int q_stride, void *q_out, int q_out_stride, const void *k, int k_stride,
                             const void *v, int v_stride, const float *rope, int n_rope);

@@ -43,3 +43,18 @@ def test_decode_workspace_is_bounded(lib, seqs, max_len, nkv, heads, hd, cache):
     most = max(64 * 256, seqs * nkv)
     assert lib.fake_ws() <= most * (heads // nkv) * (hd + 2) * 4
     assert lib.fake_blocks() <= most + seqs * heads * (hd // 32)
+
+
+@pytest.mark.parametrize("call", [append, read, decode, prompt])
+@pytest.mark.parametrize("what", [dict(table=A + 2), dict(pos=A + 1), dict(first=A + 3), dict(n_seqs=(1 << 30) + 1, n_tokens=1 << 30)])
+def test_batches_refused(lib, call, what):  # noqa: F811
+    lib.fake_reset(0)
+    assert call(lib, b=batch(**what)) == -1
+    assert lib.fake_launches() == 0 and lib.fake_error()
+
+
+@pytest.mark.parametrize("call", [append, read, decode, prompt])
+def test_batches_of_words_anywhere(lib, call):  # noqa: F811
+    """table, pos and first need no more than the alignment of their words."""
+    lib.fake_reset(0)
+    assert call(lib, b=batch(table=A + 4, pos=A + 8, first=A + 12)) == 0 and lib.fake_launches()
