@@ -478,16 +478,19 @@ int gq_hip_paged_read_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *ba
  * batch): q row first[s + 1] - 1 (row s with first NULL) over positions 0 ..
  * pos[s] + n - 1 of its cache, scaled by 1 / sqrt(head_dim), into the same row
  * of out.  q and out: n_heads x head_dim values of xtype a row; n_heads /
- * n_kv_heads from 1 to 16.  Scores, softmax and sums are fp32 throughout.  A
- * token that sees no position gets zeros; rows of no sequence stay as they
- * were.  Workspace for split sequences is the context's. */
+ * n_kv_heads from 1 to 16.  Scores, softmax and sums are fp32; under GQ_BF16
+ * queries over a GQ_BF16 or GQ_I8_ROWS cache the probabilities (times V's
+ * scales) meet V as two bf16 numbers, within 2^-17 of themselves.  A token that
+ * sees no position gets zeros; rows of no sequence stay as they were.  Workspace
+ * for split sequences is the context's, 136 MB at most on 256 CUs. */
 int gq_hip_paged_decode_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *batch, int xtype, int n_heads,
                             const void *q, int q_stride, void *out, int out_stride);
 /* The same for every new token: causal attention of packed prompts, token t of
  * sequence s over positions 0 .. pos[s] + t, whose rows are in the cache.
  * GQ_F32 queries keep fp32 accuracy throughout; with GQ_BF16 ones the
- * probabilities are rounded to bf16 before they meet V, and the values of a
- * GQ_F32 or GQ_I8_ROWS cache before they meet either.
+ * probabilities (times V's scales of a GQ_I8_ROWS cache) are rounded to bf16
+ * before they meet V, and the values of a GQ_F32 cache are two bf16 numbers
+ * each, within 2^-17 of themselves.  bf16 values and int8 codes are exact.
  * Both attentions: an infinity or NaN in the cache reaches the tokens that see
  * its position and no others.  Of V, or in the scale of its row, it makes their
  * outputs in its dimension (the row's dimensions) NaN.  Of K it makes the score
