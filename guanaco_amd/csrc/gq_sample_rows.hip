@@ -48,7 +48,7 @@ constexpr int kFine = 2048;                    /* bins of eleven bits */
 constexpr int kChunks = 16;
 constexpr int kShare = 512;                    /* tokens of the border's bin that a wave can list */
 constexpr int kList = kW * kShare;
-constexpr int kRows = 512;                     /* rows a launch: 40 MB of workspace at most */
+constexpr int kRows = 512;                     /* rows a launch: 43 MB of workspace at most */
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 

@@ -515,8 +515,12 @@ int gq_hip_paged_prompt_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *
  *   rnd          in [0, 1): the first token in index order at which the sum of
  *                the kept w passes rnd times their whole sum
  * to tokens[rows], and log(w / whole sum) to logprobs[rows] (may be NULL; 0
- * for temperature 0).  The weights and sums are exact to 2^-45 of the largest
- * and the same in every call.  NaN and -infinity are never picked; a row of
+ * for temperature 0).  A weight is a whole number of 2^-S of the largest, off by
+ * one of them at most: S = 62 - ceil(log2 vocab), 51 at most, 45 at 128256
+ * tokens and 42 at 2^20.  Sums of weights add nothing to that, in whatever
+ * order, and are the same in every call: off by vocab 2^-S of the largest weight
+ * at most, so that a draw or a border nearer to the next token may take that one.
+ * NaN and -infinity are never picked; a row of
  * nothing else gets -1 and -infinity.  Asynchronous on the context's stream;
  * workspace is the context's.
  * gq_hip_sample_dev follows the reference's samplers for one row instead:

@@ -2,7 +2,7 @@
 (tests/test_paged_host.py's stand-in for the context and HIP)."""
 import pytest
 
-from test_paged_host import A, BF16, F32, I8, append, batch, decode, lib, pages, prompt, read  # noqa: F401
+from test_paged_host import A, BF16, F32, I8, append, batch, decode, lib, pages, prompt, read, sample  # noqa: F401
 
 BIG = dict(table_stride=1 << 20)
 
@@ -58,3 +58,11 @@ def test_batches_of_words_anywhere(lib, call):  # noqa: F811
     """table, pos and first need no more than the alignment of their words."""
     lib.fake_reset(0)
     assert call(lib, b=batch(table=A + 4, pos=A + 8, first=A + 12)) == 0 and lib.fake_launches()
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 255, 256, 257, 511, 512, 5000])
+@pytest.mark.parametrize("vocab", [1000, 128256, 1 << 20])
+def test_sampling_workspace_is_bounded(lib, rows, vocab):  # noqa: F811
+    lib.fake_reset(0)
+    assert sample(lib, rows=rows, vocab=vocab, stride=vocab) == 0
+    assert 0 < lib.fake_ws() < 43.1e6
