@@ -294,8 +294,15 @@ def _ctx():
     return _shared[0]
 
 
+def _ready():
+    """The context's stream waits for no other: what torch has been given to
+    write is there before a state's first call."""
+    torch.cuda.synchronize()
+
+
 def _plan(st):
     """The descriptions of the cache and the batch that a program keeps."""
+    _ready()
     import guanaco_amd.hip as H
     c = st.case
     code = {"f32": H.S.F32, "bf16": H.BF16, "i8": H.I8_ROWS}
@@ -308,7 +315,10 @@ def _plan(st):
 def _own(st):
     c = st.case
     if c["kind"] == "sample":
-        b = st.plan = st.plan or [Buf(t) for t in (st.logits, st.temperature, st.top_k, st.top_p, st.min_p, st.rnd, st.tokens, st.logprobs)]
+        if not st.plan:
+            _ready()
+            st.plan = [Buf(t) for t in (st.logits, st.temperature, st.top_k, st.top_p, st.min_p, st.rnd, st.tokens, st.logprobs)]
+        b = st.plan
         _ctx().sample_rows_dev(b[0], c["rows"], c["vocab"], c["vocab"], *b[1:])
         return {"tokens": st.tokens, "logprobs": st.logprobs}
     ctx, pages, batch, x = st.plan = st.plan or _plan(st)
@@ -328,6 +338,8 @@ def _own(st):
 
 
 def run(st):
+    """One pass.  With `own` it runs on the context's stream: synchronise the
+    device before the outputs are read or the state is dropped or written to."""
     if own:
         return _own(st)
     kind = st.case["kind"]
