@@ -57,8 +57,9 @@ __device__ __forceinline__ int quant(float y, float d) {
  * in a page, their scales too.  Memory bounds both kernels on long batches: 8122
  * tokens of 32 + 16 bf16 rows appended in 49 us (4.3 TB/s of reads and writes),
  * 32000 int8 rows of 8 heads read as fp32 in 49 (6.7 TB/s, four fifths of it
- * writes); 32 tokens take 5.7 and 4.1, three dependent trips (sequence, page,
- * rows).  Rows read are stored past the caches (83 us if not).  Rows appended are
+ * writes).  32 tokens of as many sequences take 5.7 and 4.1, trips to memory in
+ * turn: the ends of 64 sequences, from the tile's first token's to a row's own one
+ * by one (up to 16), then its position, its page and its rows.  Rows read are stored past the caches (83 us if not).  Rows appended are
  * not, since attention reads them next: the append would take 44 us, reading 33 MB of
  * them back 17 instead of 14. */
 constexpr int kRowTile = 16;
@@ -280,8 +281,9 @@ __device__ __forceinline__ bool decode_row(const AttArgs &a, int s, int &row, in
  * The cache's bytes bound it: 64 sequences of up to 8192 positions (bf16, 32
  * heads over 8 of 128, 998 MB) 175 us with the merge, 5.7 TB/s where a copy
  * reaches 5.2; one of 131072 (int8, 277 MB) 51 us.  One of 301 takes 7.2 us: a
- * launch and four dependent trips to memory.  Eight waves a workgroup were slower
- * (64 sequences 250 us for 207 then). */
+ * launch, the trips to its row, page and keys, and five steps of 64 fp32 keys a
+ * workgroup, each waiting for loads of the one before.  Eight waves a workgroup
+ * were slower (64 sequences 250 us for 207 then). */
 template <int CT, int XT, int HD>
 __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
   constexpr int NW = kThreads / GQ_WAVE;
@@ -299,8 +301,8 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(AttArgs a) {
   bid /= a.c.n_kv;
   /* Workgroups go round the chip's engines in turn: with parts in the same order
    * for every sequence, the ones that shorter sequences lack leave the same
-   * engines idle (128 sequences to 2000: 147 us, 116 with the order turned; 64 to
-   * 8192: 202, 193). */
+   * engines idle (128 sequences to 2000: 146 us, 111 with the order turned; 64 to
+   * 8192: 185, 175). */
   const int item = bid / a.nch, part = (int)(((unsigned)bid + item + item / 2) % (unsigned)a.nch);
   /* sequence, row and length */
   const int s = item;
