@@ -88,8 +88,9 @@ __device__ __forceinline__ bool find_rows(const PgdPages &c, const PgdBatch &b, 
     }
     const bool in = t < b.n_tokens && s < b.n_seqs;
     const int sc = in ? s : 0;
-    const int r0 = b.first ? gld<int>(b.first + sc) : t, p0 = pgd_before(b, gld<int>(b.pos + sc));
-    o.t[u] = in && r0 >= 0 && t >= r0 ? t : -1;
+    const int r0 = b.first ? gld<int>(b.first + sc) : t, r1 = b.first ? gld<int>(b.first + sc + 1) : t + 1;
+    const int p0 = pgd_before(b, gld<int>(b.pos + sc));
+    o.t[u] = in && r0 >= 0 && t >= r0 && r1 <= b.n_tokens ? t : -1; /* as pgd_rows has it */
     o.p[u] = o.t[u] < 0 || p0 < 0 ? -1 : p0 + (t - r0);
     o.page[u] = o.t[u] < 0 || o.p[u] < 0 ? -1 : pgd_page(c, b, sc, o.p[u]);
   }

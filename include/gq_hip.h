@@ -440,9 +440,10 @@ typedef struct {
  * means that its positions do not exist.  pos[s] is the number of positions
  * before the call's tokens (-1: an idle slot), first[s] the row of its first
  * new token in the packed arrays of n_tokens rows, first[s + 1] - first[s]
- * their number (0 is allowed).  first NULL: one token each, row s.  max_len: no
- * sequence is longer, its new tokens included; positions from there on do not
- * exist either.  It sizes launches and workspaces, so a close bound is faster.
+ * their number (0 is allowed; a sequence whose rows are not all among the
+ * n_tokens has none).  first NULL: one token each, row s.  max_len: no sequence
+ * is longer, its new tokens included; positions from there on do not exist
+ * either.  It sizes launches and workspaces, so a close bound is faster.
  * max_len, n_tokens and n_seqs: 2^30 at most. */
 typedef struct {
   const int32_t *table, *pos, *first;
