@@ -79,17 +79,16 @@ __device__ __forceinline__ bool find_rows(const PgdPages &c, const PgdBatch &b, 
   for (int u = 0; u < U; u++) {
     const uint32_t r = w0 - t0 * per + u * RPW + sub_row;
     const int t = (int)(t0 + r % kRowTile);
-    int s = s0;
+    int s = s0, r1 = t + 1; /* the sequence's end */
     o.j[u] = (int)(r / kRowTile);
     if (t < b.n_tokens) {
       if (!b.first) s = t;
       else
-        while (s < b.n_seqs && gld<int>(b.first + s + 1) <= t) s++;
+        while (s < b.n_seqs && (r1 = gld<int>(b.first + s + 1)) <= t) s++;
     }
     const bool in = t < b.n_tokens && s < b.n_seqs;
     const int sc = in ? s : 0;
-    const int r0 = b.first ? gld<int>(b.first + sc) : t, r1 = b.first ? gld<int>(b.first + sc + 1) : t + 1;
-    const int p0 = pgd_before(b, gld<int>(b.pos + sc));
+    const int r0 = b.first ? gld<int>(b.first + sc) : t, p0 = pgd_before(b, gld<int>(b.pos + sc));
     o.t[u] = in && r0 >= 0 && t >= r0 && r1 <= b.n_tokens ? t : -1; /* as pgd_rows has it */
     o.p[u] = o.t[u] < 0 || p0 < 0 ? -1 : p0 + (t - r0);
     o.page[u] = o.t[u] < 0 || o.p[u] < 0 ? -1 : pgd_page(c, b, sc, o.p[u]);
