@@ -59,9 +59,10 @@ __device__ __forceinline__ int quant(float y, float d) {
  * 32000 int8 rows of 8 heads read as fp32 in 49 (6.7 TB/s, four fifths of it
  * writes).  32 tokens of as many sequences take 5.7 and 4.1, trips to memory in
  * turn: the ends of 64 sequences, from the tile's first token's to a row's own one
- * by one (up to 16), then its position, its page and its rows.  Rows read are stored past the caches (83 us if not).  Rows appended are
- * not, since attention reads them next: the append would take 44 us, reading 33 MB of
- * them back 17 instead of 14. */
+ * by one (up to 16), then its position, its page and its rows.  Rows read are
+ * stored past the caches (83 us if not).  Rows appended are not, since attention
+ * reads them next: the append would take 44 us, reading 33 MB of them back 17
+ * instead of 14. */
 constexpr int kRowTile = 16;
 template <int U>
 struct Rows {

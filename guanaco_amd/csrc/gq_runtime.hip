@@ -316,9 +316,9 @@ static size_t pf_held(const gq_ctx *c);
 static void paged_drop(gq_ctx *c);
 /* A request that finds no room takes back what can be made again if it fits
  * then: the prompts' workspaces, which the next one makes as the room allows,
- * that of the paged entry points, and then the bf16 copies of the weights.  Want::prompt: the caller is a
- * prompt, whose workspaces are in use.  Want::optional: it can do without too;
- * nothing is taken back. */
+ * that of the paged entry points, and then the bf16 copies of the weights.
+ * Want::prompt: the caller is a prompt, whose workspaces are in use.
+ * Want::optional: it can do without too; nothing is taken back. */
 enum class Want { must, prompt, optional };
 static void *dev_alloc(gq_ctx *c, size_t bytes, Want want = Want::must) {
   void *p = try_malloc(bytes + kPad);

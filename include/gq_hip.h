@@ -492,6 +492,7 @@ int gq_hip_paged_decode_dev(gq_ctx *ctx, const gq_pages *pages, const gq_batch *
  * probabilities (times V's scales of a GQ_I8_ROWS cache) are rounded to bf16
  * before they meet V, and the values of a GQ_F32 cache are two bf16 numbers
  * each, within 2^-17 of themselves.  bf16 values and int8 codes are exact.
+ * Workspace for long sequences is the context's, 512 MB at most.
  * Both attentions: an infinity or NaN in the cache reaches the tokens that see
  * its position and no others.  Of V, or in the scale of its row, it makes their
  * outputs in its dimension (the row's dimensions) NaN.  Of K it makes the score

@@ -66,3 +66,20 @@ def test_sampling_workspace_is_bounded(lib, rows, vocab):  # noqa: F811
     lib.fake_reset(0)
     assert sample(lib, rows=rows, vocab=vocab, stride=vocab) == 0
     assert 0 < lib.fake_ws() < 43.1e6
+
+
+@pytest.mark.parametrize("nkv,heads,hd", [(8, 32, 128), (1, 16, 64), (8, 8, 64), (8, 128, 128)])
+@pytest.mark.parametrize("cache", [F32, BF16, I8])
+@pytest.mark.parametrize("xt", [F32, BF16])
+def test_prompt_workspace_is_bounded(lib, nkv, heads, hd, cache, xt):  # noqa: F811
+    """However many tokens and whatever the bound; few tokens over many keys still
+    come in parts."""
+    p = pages(n_kv_heads=nkv, head_dim=hd, dtype=cache, page_size=1024, n_pages=1 << 20)
+    for seqs in (1, 16, 256):
+        for n in (seqs, 1000, 8000, 64000, 1000000):
+            for max_len in (1000, 32000, 131072, 1 << 30):
+                lib.fake_reset(0)
+                b = batch(n_seqs=seqs, n_tokens=n, max_len=max_len, table_stride=1 << 20)
+                assert prompt(lib, p, b, xt, nh=heads, qs=1 << 15, os=1 << 15) == 0, lib.fake_error()
+                assert lib.fake_ws() <= 512 << 20
+                assert seqs > 1 or n > 1 or max_len < 32000 or lib.fake_launches() == 2
